@@ -43,7 +43,13 @@ constexpr int S2_SLOTS = 9;
 constexpr int S2_KSTEPS = 14;            // ceil(9 * 48 / 32)
 constexpr int S2_LDS = S2_SLOTS * S2_SLOT;
 
-__device__ __forceinline__ float silu_2(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+__device__ __forceinline__ float silu_2(float v) {
+    float r = v * __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+    // the product is an f32 of its own: without this the compiler folds SOME of them into the conversion to f16 (one rounding instead
+    // of two), and which ones depends on the instructions it may use
+    asm("" : "+v"(r));
+    return r;
+}
 
 __device__ __forceinline__ void dma16_2(u32x4 rsrc, unsigned lds_addr, unsigned voff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"

@@ -7,11 +7,11 @@ R=${2:-r06}
 export TMPDIR=/tmp
 OUT=gpurun_out/round
 mkdir -p $OUT
-hipcc --offload-arch=gfx950 -O3 tools/microbench/mfma_power.hip -o /tmp/mfma_power && /tmp/mfma_power > $OUT/${R}_mfma_power_f16.txt
-hipcc --offload-arch=gfx950 -O3 tools/microbench/mfma_fp8_power.hip -o /tmp/mfma_fp8 && /tmp/mfma_fp8 > $OUT/${R}_mfma_power_fp8.txt
+hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench/mfma_power.hip -o /tmp/mfma_power && /tmp/mfma_power > $OUT/${R}_mfma_power_f16.txt
+hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench/mfma_fp8_power.hip -o /tmp/mfma_fp8 && /tmp/mfma_fp8 > $OUT/${R}_mfma_power_fp8.txt
 bash tools/conv_pmc.sh 256,40,40,192,192 800 conv_t32 > $OUT/${R}_conv_t32_pmc.txt 2>&1
 bash tools/conv_pmc.sh 256,80,80,192,384,3,2 952 conv_g32 > $OUT/${R}_conv_g32_pmc.txt 2>&1
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 tools/microbench/lds_dma_rate.hip -o /tmp/lds_dma && /tmp/lds_dma > $OUT/${R}_lds_dma_rate.txt
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/microbench/lds_dma_rate.hip -o /tmp/lds_dma && /tmp/lds_dma > $OUT/${R}_lds_dma_rate.txt
 {
   echo "# effective clock (GRBM_GUI_ACTIVE summed over 8 XCDs / duration: divide the printed GHz by 8) and MFMA-busy fraction"
   echo "# (printed fraction x 8) of one layer, M409600 N192 K1728, random operands unless noted"
