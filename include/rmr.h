@@ -408,6 +408,74 @@ rmr_status rmr_upload_begin(rmr_upload* up, int slot, const void* const* src, co
 /* blocks the calling thread until the slot's copies have landed (no-op when none is pending) */
 rmr_status rmr_upload_wait(rmr_upload* up, int slot);
 
+/* ---------------------------------------------------------------- rows of features: cache and linear layer
+ * No reference counterpart: dense operators for what a program does with the detector's features behind the detector -- keep
+ * them over frames, run one more head on them.  All tensors are DEVICE memory of the handle's device; calls are enqueued on
+ * `stream` (a hipStream_t, NULL = the default stream) and return at once; they allocate nothing and can be captured into a
+ * HIP graph.  Rows may start at any multiple of their element size and be any number of elements apart. */
+
+enum { RMR_TYPE_F16 = 0, RMR_TYPE_BF16 = 1, RMR_TYPE_F32 = 2 };
+
+/* Slots of rows of `width` values, held in 8 bits: per block of 32 values a power of two 2^e (one byte) and 32 OCP e4m3 values
+ * v / 2^e, rounded to nearest even.  e is the smallest exponent in [-127, 127] with max|v| <= 448 * 2^e over the block's finite
+ * values (-127 for zeros), so no finite value saturates; infinities and NaN are held as NaN.  A new cache holds zeros. */
+typedef struct rmr_feature_cache rmr_feature_cache;
+#define RMR_FEATURE_MAX_WIDTH 65536
+rmr_status rmr_feature_cache_create(int device, int64_t slots, int width, rmr_feature_cache** out);
+void rmr_feature_cache_destroy(rmr_feature_cache* cache);
+/* device memory it holds; 0 for NULL */
+size_t rmr_feature_cache_bytes(const rmr_feature_cache* cache);
+/* Row i of x (x + i * ld elements of `type`) enters slot slots[i] (DEVICE array of n).  A row whose slot is outside
+ * [0, slots of the cache) is left out; of several rows that name one slot the last one stays.  Calls on one cache are
+ * ordered by the caller when one of them writes (one stream, or events). */
+rmr_status rmr_feature_cache_write(rmr_feature_cache* cache, const void* x, int type, int64_t ld, const int64_t* slots, int64_t n,
+                                   void* stream);
+/* out[i] = the row in slots[i], rounded once to `type`; zeros where there is no such slot */
+rmr_status rmr_feature_cache_read(rmr_feature_cache* cache, const int64_t* slots, int64_t n, void* out, int type, int64_t ld,
+                                  void* stream);
+/* The output of backbone / neck stage `name` for image `img` of the detector's last call (rmr_detector_read_feature, under the
+ * same conditions) enters the cache without leaving the device: pixel (y, x) in slot first_slot + y * w + x.  Complete on return. */
+rmr_status rmr_detector_keep_feature(rmr_detector* det, const char* name, int img, rmr_feature_cache* cache, int64_t first_slot);
+
+/* y[i] = act(W x[i] + bias) + residual[i] in one launch, accumulated in f32 and rounded once.
+ * F16 / BF16: x and W of that type.  MX8: x and W held as a feature cache holds its rows, x quantised within the call. */
+enum { RMR_LINEAR_F16 = 0, RMR_LINEAR_BF16 = 1, RMR_LINEAR_MX8 = 2 };
+enum { RMR_ACT_NONE = 0, RMR_ACT_RELU = 1, RMR_ACT_SILU = 2, RMR_ACT_GELU = 3 /* v / 2 erfc(-v / sqrt 2) */, RMR_ACT_SIGMOID = 4 };
+typedef struct {
+    int device;
+    int in_features, out_features;
+    int format;      /* RMR_LINEAR_* */
+    int activation;  /* RMR_ACT_* */
+} rmr_linear_cfg;
+typedef struct rmr_linear rmr_linear;
+/* weight [out_features][in_features] of weight_type, rows ldw elements apart, rounded once to the layer's format and laid out
+ * for it; bias f32 [out_features] or NULL; both in `mem` (RMR_MEM_HOST / RMR_MEM_DEVICE), free again on return.  Work on
+ * `stream` that writes them is waited for. */
+rmr_status rmr_linear_create(const rmr_linear_cfg* cfg, const void* weight, int weight_type, int64_t ldw, const float* bias, int mem,
+                             void* stream, rmr_linear** out);
+void rmr_linear_destroy(rmr_linear* layer);
+/* One call's operands.  x: `rows` rows of x_type, ldx elements apart (F16 / BF16: the layer's type; MX8: any).  y, and residual
+ * if not NULL: rows of y_type, ldy / ldr elements apart.  residual may BE y (same address and ldr = ldy); apart from that y
+ * overlaps no operand, and its rows do not overlap (ldy >= out_features).  Rows are x, or -- rmr_linear_run_kept, MX8
+ * layers -- the rows of a cache of width in_features in slots[0 .. rows) (DEVICE array; zeros where there is no such slot). */
+typedef struct {
+    const void* x;
+    int x_type;
+    int64_t ldx;
+    int64_t rows;
+    const void* residual;
+    int64_t ldr;
+    void* y;
+    int y_type;
+    int64_t ldy;
+    void* workspace;        /* DEVICE, 16-byte aligned, not shared with a call that may run at the same time */
+    size_t workspace_bytes; /* at least rmr_linear_workspace of the same call */
+} rmr_linear_call;
+/* bytes of workspace that a call with these operands needs (its workspace fields are not read); kept: through rmr_linear_run_kept */
+rmr_status rmr_linear_workspace(const rmr_linear* layer, const rmr_linear_call* call, int kept, size_t* bytes);
+rmr_status rmr_linear_run(rmr_linear* layer, const rmr_linear_call* call, void* stream);
+rmr_status rmr_linear_run_kept(rmr_linear* layer, rmr_feature_cache* cache, const int64_t* slots, const rmr_linear_call* call, void* stream);
+
 /* ---------------------------------------------------------------- per-kernel profile */
 
 /* HIP-event timing of the library's own launches, on the streams they run on */

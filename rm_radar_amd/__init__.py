@@ -21,7 +21,7 @@ __all__ = ["Detector", "RobotDetector", "Locator", "Robot", "PreParam", "prepara
            "letterbox_geometry", "letterbox", "preprocess", "postprocess", "transpose",
            "conv2d", "pin_plan", "restore_detection", "device_count", "profile", "DET_DTYPE", "RmrError",
            "run_batch", "Tracker", "KalmanFilter", "SingerEKF", "auction", "TRACK_TENTATIVE", "TRACK_CONFIRMED", "TRACK_DELETED",
-           "InvalidArgument", "DeviceError", "CapacityError", "Label"]
+           "FeatureCache", "Linear", "InvalidArgument", "DeviceError", "CapacityError", "Label"]
 
 # radar::Label (src/robot/robot.h:32-45)
 Label = {"BlueHero": 0, "BlueEngineer": 1, "BlueInfantryThree": 2, "BlueInfantryFour": 3,
@@ -348,6 +348,11 @@ class Detector:
         out = np.empty(tuple(int(v) for v in dims), np.float32)
         check(lib().rmr_detector_read_feature(self._h, name.encode(), img, _lib.fp(out), _lib.ip(dims)))
         return out
+
+    def keep_feature(self, name, cache, first_slot, img=0):
+        """read_feature's stage output (same conditions), pixel by pixel into slots first_slot ... of a FeatureCache,
+        without leaving the device; complete on return."""
+        check(lib().rmr_detector_keep_feature(self._h, name.encode(), img, cache._h, first_slot))
 
     def infer(self, images, crops=None):
         """preprocess + network: the [n, 4+classes, anchors] tensor handed to postprocess."""
@@ -998,3 +1003,6 @@ class profile:
             e["flops"] += arr[i].flops
             e["bytes"] += arr[i].bytes
         return out
+
+
+from .rows import FeatureCache, Linear  # noqa: E402  (device rows: needs InvalidArgument and lib from above)

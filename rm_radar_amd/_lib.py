@@ -112,6 +112,17 @@ class KernelStat(C.Structure):
                 ("flops", C.c_double), ("bytes", C.c_double)]
 
 
+class LinearCfg(C.Structure):
+    _fields_ = [("device", C.c_int), ("in_features", C.c_int), ("out_features", C.c_int), ("format", C.c_int),
+                ("activation", C.c_int)]
+
+
+class LinearCall(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_type", C.c_int), ("ldx", C.c_int64), ("rows", C.c_int64),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p), ("y_type", C.c_int),
+                ("ldy", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # every symbol include/rmr.h declares: (restype, argtypes)
 _fp, _ip, _vp = C.POINTER(C.c_float), C.POINTER(C.c_int), C.c_void_p
 _P = C.POINTER
@@ -196,6 +207,17 @@ SYMBOLS = {
                                          _P(Robot), _ip, C.c_int]),
     "rmr_pipeline_run_streams": (C.c_int, [_vp, _P(_vp), C.c_int, _P(Image), _P(_fp), _ip, C.c_int, C.c_int, C.c_int, _ip,
                                            C.c_int, _P(Robot), _ip, C.c_int]),
+    "rmr_feature_cache_create": (C.c_int, [C.c_int, C.c_int64, C.c_int, _P(_vp)]),
+    "rmr_feature_cache_destroy": (None, [_vp]),
+    "rmr_feature_cache_bytes": (C.c_size_t, [_vp]),
+    "rmr_feature_cache_write": (C.c_int, [_vp, _vp, C.c_int, C.c_int64, _vp, C.c_int64, _vp]),
+    "rmr_feature_cache_read": (C.c_int, [_vp, _vp, C.c_int64, _vp, C.c_int, C.c_int64, _vp]),
+    "rmr_detector_keep_feature": (C.c_int, [_vp, C.c_char_p, C.c_int, _vp, C.c_int64]),
+    "rmr_linear_create": (C.c_int, [_P(LinearCfg), _vp, C.c_int, C.c_int64, _vp, C.c_int, _vp, _P(_vp)]),
+    "rmr_linear_destroy": (None, [_vp]),
+    "rmr_linear_workspace": (C.c_int, [_vp, _P(LinearCall), C.c_int, _P(C.c_size_t)]),
+    "rmr_linear_run": (C.c_int, [_vp, _P(LinearCall), _vp]),
+    "rmr_linear_run_kept": (C.c_int, [_vp, _vp, _vp, _P(LinearCall), _vp]),
     "rmr_profile_enable": (C.c_int, [C.c_int, C.c_int]),
     "rmr_profile_reset": (C.c_int, [C.c_int]),
     "rmr_profile_read": (C.c_int, [C.c_int, _P(KernelStat), C.c_int, _ip]),

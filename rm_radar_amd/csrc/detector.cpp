@@ -315,6 +315,25 @@ void Detector::infer(const rmr_image* imgs, const int* crops, int n, float* net_
         for (int i = 0; i < n; ++i) pp[i] = pp_pin(n)[i];
 }
 
+void Detector::keep_feature(const std::string& name, int img, FeatureCache& cache, int64_t first_slot) {
+    int dims[3];
+    int64_t ld = 0;
+    if (img < 0 || img >= last_n_) fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: image %d of a call with %d images", img, last_n_);
+    if (last_n_ > net_->chunk())
+        fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: the call's %d images ran in chunks of %d, only the last chunk's stage outputs are left", last_n_,
+             net_->chunk());
+    const __half* rows = net_->stage_rows(name, img, dims, ld);
+    if (!rows) fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: no stage named '%s'", name.c_str());
+    const int64_t n = (int64_t)dims[0] * dims[1];
+    if (cache.device() != ctx_.device) fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: detector and cache are on different devices");
+    if (cache.width() != dims[2])
+        fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: stage %s has %d channels, the cache's rows have %d values", name.c_str(), dims[2], cache.width());
+    if (first_slot < 0 || first_slot > cache.slots() - n)
+        fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: %lld rows from slot %lld do not fit %lld slots", (long long)n, (long long)first_slot, (long long)cache.slots());
+    cache.write_run(RowSource{rows, RMR_TYPE_F16, ld}, first_slot, n, stream_);
+    RMR_HIP(hipStreamSynchronize(stream_));
+}
+
 int Detector::read_heads(int first, int n, float* out, rmr_preparam* pp) {
     if (n == 0) return last_n_;
     if (first < 0 || n < 0 || first + n > last_n_ || !out)

@@ -6,6 +6,7 @@
 
 #include "common.h"
 #include "preprocess.h"
+#include "rows.h"
 #include "yolov8.h"
 
 namespace rmr {
@@ -49,6 +50,9 @@ class Detector {
     // Parity hook: images [first, first + n) of the LAST call's network output ([4 + classes][anchors] f32 each, the
     // tensor handed to postprocess) and their letterbox parameters; returns the number of images of that call
     int read_heads(int first, int n, float* out, rmr_preparam* pp);
+
+    // stage output `name` of image img of the last call into slots first_slot ... of a feature cache (rows.h)
+    void keep_feature(const std::string& name, int img, FeatureCache& cache, int64_t first_slot);
 
     Yolov8& net() { return *net_; }
     hipStream_t stream() { return stream_; }

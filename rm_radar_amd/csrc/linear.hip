@@ -1,0 +1,1027 @@
+// linear.hip -- y = act(x W^T + b) + residual on the matrix pipe, f32 accumulation, one rounding to y's type.
+//
+// All three formats (f16, bf16, block-scaled e4m3) are moved the same way, in K steps of 128 bytes along a row = eight chunks
+// of 16 bytes.  Lane (slot = lane & 15, g = lane >> 4) of a 16-row MFMA operand needs chunks g and g + 4 of its row: two operands
+// of 16x16x32 (16-bit types: chunk h * 4 + g is k = 32 h + 8 g ... + 7) or the two halves of one 16x16x128 (e4m3).
+//
+// Operands are swapped (D = W x): a lane ends with output features of ONE row.  The features of a group of 64 are dealt to the
+// four 16-row operands j as feature = 16 g + 4 j + i for D row 4 g + i, so that lane group g holds the 16 CONSECUTIVE features
+// 16 g ... 16 g + 15 of its row: bias, residual and y move in whole 16-byte pieces without any exchange between lanes.
+//
+// Weights are laid out once, in the order of the operand registers: [group of 64][K step][j][half][lane][16 bytes], zeros behind
+// the last feature and the last k.  A group's step is 8 KiB contiguous, copied to LDS as it is and read back at lane * 16:
+// no bank conflicts, no address arithmetic.  x is copied to LDS by rows of 128 bytes, chunk c of row r at position c ^ (r >> 1 & 7),
+// which spreads the 16 rows of a fragment read over all 64 banks.
+#include <type_traits>
+#include <utility>
+
+#include "rows_device.h"
+
+namespace rmr {
+namespace {
+
+using namespace rowsdev;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// what the kernels multiply: the three formats, and mx8 rows expanded to bf16 on their way into the matrix pipe.  Inside one
+// instruction the 8-bit products are lined up to the largest of their group and cut 13 bits below it (measured with two cancelling
+// products and a third), so the block-scaled instruction's sums are good to about 2^-13 of the largest product: far below half a
+// step of a 16-bit y (2^-9, 2^-11), not of an f32 one.  A call with f32 y takes kMx8Wide: an e4m3 value times its power of two IS a
+// bf16 value, and bf16 products are summed in full f32, at half the rate.
+enum { kF16 = RMR_LINEAR_F16, kBf16 = RMR_LINEAR_BF16, kMx8 = RMR_LINEAR_MX8, kMx8Wide };
+
+constexpr int kStepBytes = 128;      // of a row, per K step
+constexpr int kGroupStep = 8192;     // bytes of one K step of 64 output features
+
+// ------------------------------------------------------------------------------------------------ laying out the weights
+
+// feature of the group of 64 that sits in slot `slot` of operand j
+__device__ __forceinline__ int feature_of(int j, int slot) { return (slot >> 2) * 16 + j * 4 + (slot & 3); }
+
+struct PackArgs {
+    const void* w;
+    int64_t ldw;
+    int n, k, ksteps, groups;
+    unsigned char* out;
+};
+
+template <class S, class T>
+__global__ __launch_bounds__(256) void pack_weight_kernel(PackArgs a) {
+    const int64_t pieces = (int64_t)a.groups * a.ksteps * (kGroupStep / 16);
+    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < pieces; p += (int64_t)gridDim.x * 256) {
+        const int lane = (int)(p & 63), h = (int)(p >> 6) & 1, j = (int)(p >> 7) & 3;
+        const int64_t gs = p >> 9;
+        const int step = (int)(gs % a.ksteps), group = (int)(gs / a.ksteps);
+        const int64_t n = (int64_t)group * 64 + feature_of(j, lane & 15);
+        const int k = step * 64 + (h * 4 + (lane >> 4)) * 8;
+        union {
+            u32x4 u;
+            T t[8];
+        } o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o.t[i] = from_f32<T>(n < a.n && k + i < a.k ? to_f32(((const S*)a.w)[n * a.ldw + k + i]) : 0.0f);
+        *(u32x4*)(a.out + p * 16) = o.u;
+    }
+}
+
+struct PackMx8Args {
+    Mx8Rows rows;
+    int n, ksteps, groups;
+    unsigned char* out;
+    unsigned* scale;
+};
+
+__global__ __launch_bounds__(256) void pack_mx8_kernel(PackMx8Args a) {
+    const int64_t pieces = (int64_t)a.groups * a.ksteps * (kGroupStep / 16);
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = (int64_t)gridDim.x * 256;
+    for (int64_t p = first; p < pieces; p += stride) {
+        const int lane = (int)(p & 63), h = (int)(p >> 6) & 1, j = (int)(p >> 7) & 3;
+        const int64_t gs = p >> 9;
+        const int step = (int)(gs % a.ksteps), group = (int)(gs / a.ksteps);
+        const int64_t n = (int64_t)group * 64 + feature_of(j, lane & 15);
+        u32x4 v = {0, 0, 0, 0};
+        if (n < a.n) v = *(const u32x4*)(a.rows.data + n * a.rows.pitch + step * kStepBytes + (h * 4 + (lane >> 4)) * 16);
+        *(u32x4*)(a.out + p * 16) = v;
+    }
+    const int quads = (a.ksteps + 3) / 4;
+    const int64_t words = (int64_t)a.groups * quads * 256;
+    for (int64_t p = first; p < words; p += stride) {
+        const int lane = (int)(p & 63), j = (int)(p >> 6) & 3;
+        const int64_t gq = p >> 8;
+        const int quad = (int)(gq % quads), group = (int)(gq / quads);
+        const int64_t n = (int64_t)group * 64 + feature_of(j, lane & 15);
+        a.scale[p] = n < a.n ? *(const unsigned*)(a.rows.scale + n * a.rows.scale_pitch + quad * 16 + (lane >> 4) * 4) : 0u;
+    }
+}
+
+// rows of 16-bit values to rows of `pitch` bytes, zeros behind the last value: for rows whose length or alignment does not
+// allow 16-byte pieces
+struct AlignArgs {
+    const void* x;
+    int64_t ld, n;
+    int width, per_row;
+    unsigned char* out;
+};
+
+__global__ __launch_bounds__(256) void align_rows_kernel(AlignArgs a) {
+    const int64_t pieces = a.n * a.per_row;
+    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < pieces; p += (int64_t)gridDim.x * 256) {
+        const int64_t r = p / a.per_row;
+        const int c = (int)(p - r * a.per_row) * 8;
+        const unsigned short* src = (const unsigned short*)a.x + r * a.ld + c;
+        union {
+            u32x4 u;
+            unsigned short t[8];
+        } o;
+        if (c + 8 <= a.width) {
+            o.u = *(const u32x4_any*)src;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.t[i] = c + i < a.width ? src[i] : (unsigned short)0;
+        }
+        *(u32x4*)(a.out + p * 16) = o.u;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------- the epilogue
+
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+    if constexpr (ACT == RMR_ACT_RELU) return v < 0.0f ? 0.0f : v;
+    if constexpr (ACT == RMR_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+    if constexpr (ACT == RMR_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+    if constexpr (ACT == RMR_ACT_GELU) {
+        // v / 2 erfc(-v / sqrt 2) with Abramowitz & Stegun 7.1.26: erfc(z) = t (a1 + t (a2 + ...)) e^(-z z), t = 1 / (1 + p z), z >= 0,
+        // off by at most 1.5e-7 absolutely, which is 0.75e-7 |v| here
+        const float z = fabsf(v) * 0.70710678f;
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
+        float q = fmaf(1.061405429f, t, -1.453152027f);
+        q = fmaf(q, t, 1.421413741f);
+        q = fmaf(q, t, -0.284496736f);
+        q = fmaf(q, t, 0.254829592f);
+        q *= t * __expf(-z * z);                       // erfc(|v| / sqrt 2)
+        const float h = 0.5f * v;
+        return v < 0.0f ? h * q : h * (2.0f - q);
+    }
+    return v;
+}
+
+struct LinearArgs {
+    // rows: chunk c of row i at x + (slots ? slots[i] : i) * x_pitch + c * 16
+    const unsigned char* x;
+    int64_t x_pitch;
+    const unsigned char* x_scale;   // mx8
+    int64_t x_scale_pitch;
+    const int64_t* slots;
+    int64_t n_slots;
+    int64_t rows;
+    int last_chunks;   // 16-byte chunks of a row that the last K step has
+    const unsigned char* zero;
+    const unsigned char* w;
+    const unsigned* w_scale;
+    const float* bias;
+    int ksteps, groups, out_features;
+    const void* residual;
+    int64_t ldr;
+    void* y;
+    int64_t ldy;
+    int y_type, act;
+    int wide;   // y and residual move in 16-byte pieces
+    int64_t row_tiles;
+    int col_tiles;
+};
+
+template <class T>
+__device__ __forceinline__ void store_row(const LinearArgs& a, const f32x4 (&v)[4], int64_t row, int c0, int have) {
+    constexpr int V = 16 / (int)sizeof(T);
+    T* y = (T*)a.y + row * a.ldy + c0;
+    const T* r = a.residual ? (const T*)a.residual + row * a.ldr + c0 : nullptr;
+#pragma unroll
+    for (int p = 0; p < 16 / V; ++p) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = v[(p * V + i) >> 2][(p * V + i) & 3];
+        if (r) {
+            float rv[V];
+            load_values<T>(r + p * V, have - p * V, rv);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] += rv[i];
+        }
+        store_values<T>(y + p * V, have - p * V, o);
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void activate_row(f32x4 (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = activate<ACT>(v[j][i]);
+}
+
+// 16 features c0 ... of one row: v[j][i] is feature c0 + 4 j + i before the bias
+__device__ __forceinline__ void finish_row(const LinearArgs& a, f32x4 (&v)[4], const f32x4 (&bias)[4], int64_t row, int c0) {
+    const int have = a.out_features - c0;
+    if (row >= a.rows || have <= 0) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += bias[j];
+    switch (a.act) {
+        case RMR_ACT_RELU: activate_row<RMR_ACT_RELU>(v); break;
+        case RMR_ACT_SILU: activate_row<RMR_ACT_SILU>(v); break;
+        case RMR_ACT_GELU: activate_row<RMR_ACT_GELU>(v); break;
+        case RMR_ACT_SIGMOID: activate_row<RMR_ACT_SIGMOID>(v); break;
+        default: break;
+    }
+    if (a.y_type == RMR_TYPE_F16)
+        store_row<F16>(a, v, row, c0, have);
+    else if (a.y_type == RMR_TYPE_BF16)
+        store_row<BF16>(a, v, row, c0, have);
+    else
+        store_row<float>(a, v, row, c0, have);
+}
+
+// ------------------------------------------------------------------------------------------------------- the tile kernel
+
+// f(integral_constant<K>) ... f(integral_constant<N - 1>)
+template <int K, int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (K < N) {
+        f(std::integral_constant<int, K>{});
+        static_for<K + 1, N>(std::forward<F>(f));
+    }
+}
+
+// 64 lanes x 16 bytes of global memory to LDS at lds + lane * 16 where `mask` is -1, nothing where it is 0 (uniform; the wave's 64
+// lanes are all active here)
+__device__ __forceinline__ void dma_lane(unsigned lds, const unsigned char* p, int mask) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b64 exec, -1"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p), "s"(__builtin_amdgcn_readfirstlane(mask))
+                 : "memory");
+}
+// the same from a uniform address + lane offset
+__device__ __forceinline__ void dma_uniform(unsigned lds, const unsigned char* base, unsigned off, int mask) {
+    const uint64_t b = (uint64_t)base;
+    const uint64_t u = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(b >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((unsigned)b);
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(u), "s"(__builtin_amdgcn_readfirstlane(mask))
+                 : "memory");
+}
+
+// 16 e4m3 values times 2^(byte - 127) as two bf16 operands, values 0 ... 7 and 8 ... 15
+__device__ __forceinline__ void widen(u32x4 v, unsigned byte, bf16x8 (&o)[2]) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const float scale = __uint_as_float(byte << 23);   // the conversion takes the exponent field only
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], scale, false);
+        const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], scale, true);
+        o[i >> 1][(i & 1) * 4 + 0] = lo[0], o[i >> 1][(i & 1) * 4 + 1] = lo[1];
+        o[i >> 1][(i & 1) * 4 + 2] = hi[0], o[i >> 1][(i & 1) * 4 + 3] = hi[1];
+    }
+}
+
+// one operand of a K step in the registers it is multiplied from
+template <int FORMAT>
+struct Operand {
+    u32x4 h[2];
+    unsigned scale;
+    __device__ __forceinline__ void set(const u32x4 (&v)[2], const unsigned (&s)[2]) { h[0] = v[0], h[1] = v[1], scale = s[0]; }
+};
+template <>
+struct Operand<kMx8Wide> {
+    bf16x8 b[2][2];
+    __device__ __forceinline__ void set(const u32x4 (&v)[2], const unsigned (&s)[2]) { widen(v[0], s[0] & 255, b[0]), widen(v[1], s[1] & 255, b[1]); }
+};
+
+template <int FORMAT>
+__device__ __forceinline__ f32x4 step_product(const Operand<FORMAT>& w, const Operand<FORMAT>& x, f32x4 c) {
+    if constexpr (FORMAT == kF16) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w.h[h]), __builtin_bit_cast(half8, x.h[h]), c, 0, 0, 0);
+    } else if constexpr (FORMAT == kBf16) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.h[h]), __builtin_bit_cast(bf16x8, x.h[h]), c, 0, 0, 0);
+    } else if constexpr (FORMAT == kMx8) {
+        struct Two {
+            u32x4 h[2];
+        };
+        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, Two{{w.h[0], w.h[1]}}),
+                                                             __builtin_bit_cast(i32x8, Two{{x.h[0], x.h[1]}}), c, 0, 0, 0, (int)w.scale, 0, (int)x.scale);
+    } else {
+        // both operands deal their 128 values to the four instructions alike, so the order along k does not matter
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.b[h][i], x.b[h][i], c, 0, 0, 0);
+    }
+    return c;
+}
+
+// scale dwords a lane holds per row: its own block's, or -- widened -- those of the blocks its two chunks lie in
+template <int FORMAT>
+constexpr int kScales = FORMAT == kMx8Wide ? 2 : 1;
+template <int FORMAT>
+__device__ __forceinline__ int scale_block(int h, int g) {
+    return FORMAT == kMx8Wide ? h * 2 + (g >> 1) : g;
+}
+
+// One tile of 16 MT WM rows x 64 G WN features; a wave computes 16 MT x 64 G.
+//
+// Two LDS buffers of one K step each.  A step has two (or four) phases, parts of its rows.  While one part multiplies, the next part's
+// fragments are read from LDS; before the last part every read of the buffer is done, one barrier, and while the last part
+// multiplies the copies of step t + 2 go out into this buffer and the first fragments of step t + 1 come in from the other one.  So
+// a copy has a whole step to land, a fragment a phase, and a step costs one barrier.  Everything that is not a product is dealt
+// evenly over the products of its phase (sched_barrier keeps it there): the matrix pipe runs while the rest issues in its shadow.
+template <int FORMAT, int MT, int G, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_tile_kernel(LinearArgs a) {
+    constexpr bool kScaled = FORMAT == kMx8 || FORMAT == kMx8Wide;
+    constexpr int S = kScales<FORMAT>;
+    constexpr int NP = FORMAT == kMx8 && MT == 8 ? 4 : 2;   // phases of a step (four: half the registers for rows)
+    constexpr int kWaves = WM * WN, MH = MT / NP, J = 4 * G;
+    constexpr int BM = 16 * MT * WM, BG = G * WN;
+    constexpr int kXBytes = BM * kStepBytes, kWBytes = BG * kGroupStep;
+    constexpr int kXPer = BM / 8 / kWaves;               // copies of 8 rows per wave and step
+    constexpr int kWPer = BG * 8 / kWaves;               // copies of 1 KiB of weights per wave and step
+    constexpr int kXScale = (BM + 63) / 64 * 1024, kWScale = BG * 1024;   // bytes of four steps' scales
+    constexpr int kScalePieces = kXScale / 1024 + BG;
+    static_assert(BM % (8 * kWaves) == 0 && (BG * 8) % kWaves == 0 && MT % NP == 0 && kScalePieces <= 2 * kWaves, "copies divide over the waves");
+    constexpr int kW0 = 2 * kXBytes, kS0 = kW0 + 2 * kWBytes;   // LDS: both buffers' rows, both buffers' weights, two quads of scales
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kS0 + (kScaled ? 2 * (kXScale + kWScale) : 0)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+    // consecutive workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, walked in bands of kBand row tiles, so that
+    // the tiles that run on it at one time share rows and weights in its L2
+    constexpr int kBand = 8;
+    int64_t mt;
+    int nt;
+    {
+        const unsigned tiles = gridDim.x, xcd = blockIdx.x & 7, q = tiles >> 3, r = tiles & 7;
+        const unsigned tile = xcd * q + (xcd < r ? xcd : r) + (blockIdx.x >> 3);
+        const unsigned band = tile / (kBand * a.col_tiles), in = tile - band * (kBand * a.col_tiles);
+        const unsigned left = (unsigned)a.row_tiles - band * kBand, high = left < kBand ? left : kBand;
+        mt = band * kBand + in % high, nt = (int)(in / high);
+    }
+    const int64_t m0 = mt * BM;
+    const int g0 = nt * BG;   // first group of 64 features
+
+    const auto source_row = [&](int lr, bool& there) {
+        int64_t row = m0 + lr;
+        if (row >= a.rows) row = a.rows - 1;   // rows behind the end repeat the last one, nothing of them is stored
+        there = true;
+        if (a.slots) {
+            row = a.slots[row];
+            there = row >= 0 && row < a.n_slots;
+        }
+        return row;
+    };
+    // ---- what this lane copies: rows (wave * kXPer + i) * 8 + lane / 8, chunk (lane & 7) ^ (row >> 1 & 7)
+    const unsigned char* xp[kXPer];
+    int xinc[kXPer];
+    unsigned tail = 0;   // bit i: copy i's chunk lies behind the row's end in the last step
+#pragma unroll
+    for (int i = 0; i < kXPer; ++i) {
+        const int lr = (wave * kXPer + i) * 8 + (lane >> 3);
+        const int chunk = (lane & 7) ^ ((lr >> 1) & 7);
+        bool there;
+        const int64_t row = source_row(lr, there);
+        xp[i] = there ? a.x + row * a.x_pitch + chunk * 16 : a.zero + chunk * 16;
+        xinc[i] = there ? kStepBytes : 0;
+        tail |= chunk >= a.last_chunks ? 1u << i : 0u;
+    }
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+    const unsigned ldsx = __builtin_amdgcn_readfirstlane(lds0 + wave * kXPer * 1024), ldsw = __builtin_amdgcn_readfirstlane(lds0 + kW0 + wave * kWPer * 1024);
+    const unsigned woff = lane * 16;
+    // a wave's pieces of 1 KiB of weights: a run of kWPer, inside one group or whole groups
+    static_assert(kWPer % 8 == 0 || 8 % kWPer == 0, "a wave's weight pieces do not straddle groups unevenly");
+    constexpr int kWGroups = (kWPer + 7) / 8;
+    const unsigned char* wp[kWGroups];
+#pragma unroll
+    for (int i = 0; i < kWGroups; ++i) {
+        int gr = g0 + wave * kWPer / 8 + i;
+        if (gr >= a.groups) gr = a.groups - 1;
+        wp[i] = a.w + ((int64_t)gr * a.ksteps * 8 + wave * kWPer % 8) * 1024;
+    }
+    // step `t`'s copies go out in order of t: the pointers walk along
+    const auto copy_x = [&](int i, int buf, int mask) {
+        dma_lane(ldsx + buf * kXBytes + i * 1024, xp[i], mask);
+        xp[i] += xinc[i];
+    };
+    const auto copy_w = [&](int i, int buf, int mask) {
+        dma_uniform(ldsw + buf * kWBytes + i * 1024, wp[i / 8] + (i % 8) * 1024, woff, mask);
+        if (i % 8 == 7 || i == kWPer - 1) wp[i / 8] += kGroupStep;
+    };
+    const auto before_copies = [&](int t) {   // the last step of rows that end inside it: what lies behind is read as zero
+        if (t == a.ksteps - 1 && a.last_chunks < 8) {
+#pragma unroll
+            for (int i = 0; i < kXPer; ++i)
+                if (tail >> i & 1) xp[i] = a.zero;
+        }
+    };
+    // four steps' scales: 64 rows' 16 bytes, or a group's 1 KiB, per copy; piece wave + k * kWaves
+    constexpr int kScalePer = kScaled ? (kScalePieces + kWaves - 1) / kWaves : 1;
+    const int quads = (a.ksteps + 3) / 4;
+    const unsigned char* sp[kScalePer];
+    int sinc[kScalePer];
+    if constexpr (kScaled) {
+#pragma unroll
+        for (int k = 0; k < kScalePer; ++k) {
+            const int piece = wave + k * kWaves;
+            if (piece < kXScale / 1024) {
+                bool there;
+                const int lr = piece * 64 + lane;
+                const int64_t row = source_row(lr < BM ? lr : BM - 1, there);
+                sp[k] = there ? a.x_scale + row * a.x_scale_pitch : a.zero;
+                sinc[k] = there ? 16 : 0;
+            } else {
+                int gr = g0 + piece - kXScale / 1024;
+                if (gr >= a.groups) gr = a.groups - 1;
+                sp[k] = (const unsigned char*)(a.w_scale + (int64_t)gr * quads * 256 + lane * 4);
+                sinc[k] = 1024;
+            }
+        }
+    }
+    const auto copy_scales = [&](int quad, int mask) {
+        if constexpr (kScaled) {
+#pragma unroll
+            for (int k = 0; k < kScalePer; ++k) {
+                const int piece = wave + k * kWaves;
+                dma_lane(lds0 + kS0 + (quad & 1) * (kXScale + kWScale) + piece * 1024, sp[k], piece < kScalePieces ? mask : 0);
+                sp[k] += mask ? sinc[k] : 0;
+            }
+        }
+    };
+
+    // ---- fragments and their scales
+    u32x4 wr[J][2], xr[2][MH][2];
+    unsigned ws[kScaled ? J : 1][2], xs[kScaled ? 2 * MH : 1][2];
+    const int xlane = (wm * MT * 16 + (lane & 15)) * kStepBytes, swz = ((lane & 15) >> 1) & 7;
+    int xl0 = xlane + ((g ^ swz) * 16), xl1 = xlane + (((4 + g) ^ swz) * 16);   // in the buffer that is read
+    int wl = kW0 + wn * G * kGroupStep + lane * 16;
+    const auto read_x = [&](int m, int h) { return *(const u32x4*)(smem + (h ? xl1 : xl0) + m * 16 * kStepBytes); };
+    const auto read_w = [&](int j, int h) { return *(const u32x4*)(smem + wl + (j >> 2) * kGroupStep + ((j & 3) * 2 + h) * 1024); };
+    // (a scale is one byte: its block's dword, the byte of the step)
+    int xsl[2], wsl[2];
+#pragma unroll
+    for (int h = 0; h < S; ++h) {
+        const int b = scale_block<FORMAT>(h, g);
+        xsl[h] = kS0 + (wm * MT * 16 + (lane & 15)) * 16 + b * 4;
+        wsl[h] = kS0 + kXScale + wn * G * 1024 + (b * 16 + (lane & 15)) * 4;
+    }
+    const auto scale_at = [&](int t) { return ((t >> 2) & 1) * (kXScale + kWScale) + (t & 3); };
+    const auto read_xs = [&](int at, int to, int m) {
+        if constexpr (kScaled)
+#pragma unroll
+            for (int h = 0; h < S; ++h) xs[to][h] = *(smem + xsl[h] + at + m * 256);
+    };
+    const auto read_ws = [&](int at, int j) {
+        if constexpr (kScaled)
+#pragma unroll
+            for (int h = 0; h < S; ++h) ws[j][h] = *(smem + wsl[h] + at + (j >> 2) * 1024 + (j & 3) * 256);
+    };
+
+    f32x4 acc[MT][J];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[m][j] = f32x4{0, 0, 0, 0};
+
+    // ---- the first two steps' copies, the first fragments
+    const auto copy_step = [&](int t, int buf) {
+        before_copies(t);
+#pragma unroll
+        for (int i = 0; i < kXPer; ++i) copy_x(i, buf, -1);
+#pragma unroll
+        for (int i = 0; i < kWPer; ++i) copy_w(i, buf, -1);
+    };
+    copy_scales(0, -1);
+    copy_step(0, 0);
+    if (a.ksteps > 1) {
+        copy_step(1, 1);
+        asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kXPer + kWPer) : "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    }
+    asm volatile("s_barrier" : : : "memory");
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) wr[j][h] = read_w(j, h);
+#pragma unroll
+        for (int m = 0; m < MH; ++m) xr[0][m][h] = read_x(m, h);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) read_ws(0, j);
+#pragma unroll
+    for (int m = 0; m < MH; ++m) read_xs(0, m, m);
+
+    // one step an iteration: every accumulator is updated once, and stays in its registers
+    for (int t = 0; t < a.ksteps; ++t) {
+        constexpr int kSlots = MH * J;   // products of a phase, the features outside, the rows inside
+        const int buf = t & 1;
+        const int now = kScaled ? scale_at(t) : 0, next = kScaled ? scale_at(t + 1) : 0;
+        const auto product = [&](auto phase, auto slot) {
+            constexpr int PH = decltype(phase)::value, m = decltype(slot)::value % MH, j = decltype(slot)::value / MH;
+            Operand<FORMAT> wf, xf;
+            const unsigned none[2] = {0, 0};
+            if constexpr (kScaled) {
+                wf.set(wr[j], ws[j]), xf.set(xr[PH & 1][m], xs[(PH & 1) * MH + m]);
+            } else {
+                wf.set(wr[j], none), xf.set(xr[PH & 1][m], none);
+            }
+            acc[PH * MH + m][j] = step_product<FORMAT>(wf, xf, acc[PH * MH + m][j]);
+        };
+        // the rows' fragments of phase `to`, dealt over the first half of the phase before it
+        const auto read_rows = [&](auto to, auto slot, int at) {
+            constexpr int T = decltype(to)::value, s = decltype(slot)::value;
+            static_for<0, 2 * MH>([&](auto act) {
+                constexpr int i = decltype(act)::value;
+                if constexpr (i * (kSlots / 2) / (2 * MH) == s) {
+                    xr[T & 1][i >> 1][i & 1] = read_x(T * MH + (i >> 1), i & 1);
+                    if constexpr (i % 2) read_xs(at, (T & 1) * MH + (i >> 1), T * MH + (i >> 1));
+                }
+            });
+        };
+        static_for<0, NP - 1>([&](auto phase) {
+            static_for<0, kSlots>([&](auto slot) {
+                product(phase, slot);
+                read_rows(std::integral_constant<int, decltype(phase)::value + 1>{}, slot, now);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        });
+        // step t + 1 has landed for every wave, and every wave has read all of step t
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+        const int more = t + 2 < a.ksteps ? -1 : 0;
+        xl0 += buf ? -kXBytes : kXBytes, xl1 += buf ? -kXBytes : kXBytes, wl += buf ? -kWBytes : kWBytes;
+        before_copies(t + 2);
+        copy_scales((t >> 2) + 1, (t & 3) == 1 && (t >> 2) + 1 < quads ? -1 : 0);
+        // last phase: the next step's first fragments -- a weight fragment right behind the last product of the one it replaces -- and
+        // the copies of the step after it
+        static_for<0, kSlots>([&](auto slot) {
+            constexpr int s = decltype(slot)::value;
+            product(std::integral_constant<int, NP - 1>{}, slot);
+            read_rows(std::integral_constant<int, 0>{}, slot, next);
+            if constexpr (s % MH == MH - 1) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) wr[s / MH][h] = read_w(s / MH, h);
+                read_ws(next, s / MH);
+            }
+            constexpr int kCopies = kXPer + kWPer;
+            static_for<0, kCopies>([&](auto act) {
+                constexpr int i = decltype(act)::value;
+                if constexpr (i * kSlots / kCopies == s) {
+                    if constexpr (i < kXPer)
+                        copy_x(i, buf, more);
+                    else
+                        copy_w(i - kXPer, buf, more);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+
+    static_for<0, G>([&](auto group) {
+        constexpr int q = decltype(group)::value;
+        const int gr = g0 + wn * G + q;
+        if (gr >= a.groups) return;
+        const int c0 = gr * 64 + g * 16;
+        f32x4 bias[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = *(const f32x4*)(a.bias + c0 + j * 4);
+        static_for<0, MT>([&](auto mm) {
+            constexpr int m = decltype(mm)::value;
+            f32x4 v[4] = {acc[m][q * 4], acc[m][q * 4 + 1], acc[m][q * 4 + 2], acc[m][q * 4 + 3]};
+            finish_row(a, v, bias, m0 + wm * MT * 16 + m * 16 + (lane & 15), c0);
+        });
+    });
+}
+
+// ---------------------------------------------------------------------------------------------------- the few-rows kernel
+//
+// Up to 16 MT rows: the weights' bytes are the work, and every one of them goes from memory straight into the registers it is
+// multiplied from -- no LDS, no barrier until the end.  A workgroup owns 16 JN features; its eight waves deal the K steps among
+// themselves (wave v takes steps v, v + 8, ...), each with kFewUnroll steps' loads in flight, and their sums are joined through LDS
+// in wave order, so the result does not depend on timing.  x is read as it is -- any alignment and length -- and quantised in
+// registers where the format asks for it: no launch in front, no workspace.
+
+constexpr int kFewWaves = 8;
+
+// where a lane's chunk of 16 bytes (of the operand) comes from
+enum { kRaw, kFromF16, kFromBf16, kFromF32, kHeld };
+template <int SRC>
+struct SourceType {
+    typedef unsigned short T;
+};
+template <>
+struct SourceType<kFromF16> {
+    typedef F16 T;
+};
+template <>
+struct SourceType<kFromBf16> {
+    typedef BF16 T;
+};
+template <>
+struct SourceType<kFromF32> {
+    typedef float T;
+};
+
+struct FewArgs {
+    LinearArgs a;
+    const void* x;   // kRaw, kFrom*: the caller's rows
+    int64_t ldx;
+    int in_features;
+};
+
+// 16 bytes of a row's values, k0 on; zeros behind its end
+template <class T>
+__device__ __forceinline__ u32x4 load_piece(const T* row, int k0, int k) {
+    constexpr int V = 16 / (int)sizeof(T);
+    if (k0 + V <= k) return *(const u32x4_any*)(row + k0);
+    union {
+        u32x4 u;
+        T t[V];
+    } o;
+    o.u = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (k0 + i < k) o.t[i] = row[k0 + i];
+    return o.u;
+}
+
+// 16 values of a row as e4m3, and their block's exponent byte.  The block's other half is in lane ^ 16.
+template <class T>
+__device__ __forceinline__ u32x4 quantised_chunk(const u32x4 (&raw)[sizeof(T)], unsigned& byte) {
+    constexpr int V = 16 / (int)sizeof(T);
+    float v[16];
+#pragma unroll
+    for (int p = 0; p < (int)sizeof(T); ++p) {
+        union {
+            u32x4 u;
+            T t[V];
+        } o;
+        o.u = raw[p];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[p * V + i] = to_f32(o.t[i]);
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float m = fabsf(v[i]);
+        top = is_finite(m) && m > top ? m : top;
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    const int e = mx8_exponent(top);
+    byte = (unsigned)(e + 127);
+    const float inv = mx8_inverse(e);
+    u32x4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = to_e4m3x4(v + 4 * i, inv);
+    return q;
+}
+
+template <class T>
+__device__ __forceinline__ void finish_quad(const LinearArgs& a, f32x4 v, int64_t row, int c0) {
+    const int have = a.out_features - c0;
+    if (row >= a.rows || have <= 0) return;
+    const f32x4 b = *(const f32x4*)(a.bias + c0);
+    v += b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        switch (a.act) {
+            case RMR_ACT_RELU: v[i] = activate<RMR_ACT_RELU>(v[i]); break;
+            case RMR_ACT_SILU: v[i] = activate<RMR_ACT_SILU>(v[i]); break;
+            case RMR_ACT_GELU: v[i] = activate<RMR_ACT_GELU>(v[i]); break;
+            case RMR_ACT_SIGMOID: v[i] = activate<RMR_ACT_SIGMOID>(v[i]); break;
+            default: break;
+        }
+    }
+    T* y = (T*)a.y + row * a.ldy + c0;
+    const T* r = a.residual ? (const T*)a.residual + row * a.ldr + c0 : nullptr;
+    if (have >= 4 && sizeof(T) == 4) {
+        if (r) {
+            float rv[4];
+            load_values<float, 4>((const float*)r, 4, rv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += rv[i];
+        }
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        store_values<float, 4>((float*)y, 4, o);
+        return;
+    }
+    if (have >= 4) {
+        union {
+            u32x2 u;
+            T t[4];
+        } w;
+        if (r) {
+            w.u = *(const u32x2_any*)r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += to_f32(w.t[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.t[i] = from_f32<T>(v[i]);
+        *(u32x2_any*)y = w.u;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < have) y[i] = from_f32<T>(v[i] + (r ? to_f32(r[i]) : 0.0f));
+}
+
+template <int FORMAT, int SRC, int MT, int JN, int U>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(FewArgs f) {
+    const LinearArgs& a = f.a;
+    constexpr bool kScaled = FORMAT == kMx8 || FORMAT == kMx8Wide;
+    constexpr int S = kScales<FORMAT>;
+    __shared__ f32x4 part[kFewWaves][MT * JN][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4;
+    const int group = blockIdx.x / (4 / JN), j0 = (blockIdx.x % (4 / JN)) * JN;
+    const unsigned char* w = a.w + ((int64_t)group * a.ksteps * 8 + j0 * 2) * 1024 + lane * 16;
+    const int quads = (a.ksteps + 3) / 4;
+    const unsigned* wsp = kScaled ? a.w_scale + (int64_t)group * quads * 256 + j0 * 64 + (lane & 15) : nullptr;
+    typedef typename SourceType<SRC>::T T;
+    constexpr bool kQuantise = SRC == kFromF16 || SRC == kFromBf16 || SRC == kFromF32;
+    constexpr int R = kQuantise ? (int)sizeof(T) : 1;   // pieces of 16 bytes that a chunk of the operand is made of
+    const T* xrow[MT];
+    const unsigned char* held[MT];
+    const unsigned char* hscale[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        int64_t row = m * 16 + (lane & 15);
+        if (row >= a.rows) row = a.rows - 1;
+        if constexpr (SRC == kHeld) {
+            row = a.slots[row];
+            const bool there = row >= 0 && row < a.n_slots;
+            held[m] = there ? a.x + row * a.x_pitch : nullptr;
+            hscale[m] = a.x_scale + row * a.x_scale_pitch;
+        } else {
+            xrow[m] = (const T*)f.x + row * f.ldx;
+        }
+    }
+    f32x4 acc[MT][JN];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < JN; ++j) acc[m][j] = f32x4{0, 0, 0, 0};
+
+    for (int t0 = wave; t0 < a.ksteps; t0 += kFewWaves * U) {
+        u32x4 wv[U][JN][2];
+        unsigned wsv[U][JN][2];
+        u32x4 xv[U][MT][2][R];
+        unsigned xsv[U][MT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = t0 + u * kFewWaves < a.ksteps ? t0 + u * kFewWaves : a.ksteps - 1;   // behind the end: loaded, not used
+#pragma unroll
+            for (int j = 0; j < JN; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) wv[u][j][h] = *(const u32x4*)(w + (int64_t)t * kGroupStep + (j * 2 + h) * 1024);
+                if constexpr (kScaled)
+#pragma unroll
+                    for (int h = 0; h < S; ++h) wsv[u][j][h] = wsp[(t >> 2) * 256 + j * 64 + scale_block<FORMAT>(h, g) * 16] >> ((t & 3) * 8);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int chunk = h * 4 + g;
+                    if constexpr (SRC == kRaw) {
+                        xv[u][m][h][0] = load_piece<T>(xrow[m], t * 64 + chunk * 8, f.in_features);
+                    } else if constexpr (SRC == kHeld) {
+                        xv[u][m][h][0] = u32x4{0, 0, 0, 0};
+                        if (held[m]) xv[u][m][h][0] = *(const u32x4*)(held[m] + t * kStepBytes + chunk * 16);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < R; ++p) xv[u][m][h][p] = load_piece<T>(xrow[m], t * kStepBytes + chunk * 16 + p * (16 / R), f.in_features);
+                    }
+                }
+                if constexpr (SRC == kHeld)
+#pragma unroll
+                    for (int h = 0; h < S; ++h)
+                        xsv[u][m][h] = held[m] ? *(const unsigned*)(hscale[m] + (t >> 2) * 16 + scale_block<FORMAT>(h, g) * 4) >> ((t & 3) * 8) : 0u;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (t0 + u * kFewWaves >= a.ksteps) break;
+            Operand<FORMAT> wf[JN];
+#pragma unroll
+            for (int j = 0; j < JN; ++j) wf[j].set(wv[u][j], wsv[u][j]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                u32x4 v[2];
+                unsigned xs[2] = {0, 0};
+                if constexpr (kQuantise) {
+                    unsigned b[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) v[h] = quantised_chunk<T>(xv[u][m][h], b[h]);
+                    if constexpr (FORMAT == kMx8Wide) {
+                        xs[0] = b[0], xs[1] = b[1];
+                    } else {
+                        // lane group g scales block g, whose two chunks 2 g and 2 g + 1 lie in half g / 2 of groups 2 g % 4 and one more
+                        const unsigned both = __shfl(b[0] | b[1] << 8, (lane & 15) + ((g & 1) << 5));
+                        xs[0] = g >> 1 ? both >> 8 : both & 255;
+                    }
+                } else {
+                    v[0] = xv[u][m][0][0], v[1] = xv[u][m][1][0];
+                    if constexpr (kScaled) xs[0] = xsv[u][m][0], xs[1] = xsv[u][m][S - 1];
+                }
+                Operand<FORMAT> xf;
+                xf.set(v, xs);
+#pragma unroll
+                for (int j = 0; j < JN; ++j) acc[m][j] = step_product<FORMAT>(wf[j], xf, acc[m][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < JN; ++j) part[wave][m * JN + j][lane] = acc[m][j];
+    __syncthreads();
+    for (int p = wave; p < MT * JN; p += kFewWaves) {
+        f32x4 v = part[0][p][lane];
+#pragma unroll
+        for (int k = 1; k < kFewWaves; ++k) v += part[k][p][lane];
+        const int64_t row = (p / JN) * 16 + (lane & 15);
+        const int c0 = group * 64 + g * 16 + (j0 + p % JN) * 4;
+        if (a.y_type == RMR_TYPE_F16)
+            finish_quad<F16>(a, v, row, c0);
+        else if (a.y_type == RMR_TYPE_BF16)
+            finish_quad<BF16>(a, v, row, c0);
+        else
+            finish_quad<float>(a, v, row, c0);
+    }
+}
+
+// rows up to which the few-rows kernel takes a call
+constexpr int64_t kFewRows = 32;
+
+template <int FORMAT, int SRC>
+void launch_few(const FewArgs& f, hipStream_t s) {
+    // steps in flight: what fits the registers without spilling
+    constexpr int U1 = SRC == kFromF32 ? 2 : 4, U2 = SRC == kFromF32 ? 1 : SRC == kFromF16 || SRC == kFromBf16 ? 2 : 4;
+    const unsigned grid = (unsigned)f.a.groups * 4;
+    if (f.a.rows <= 16)
+        linear_few_kernel<FORMAT, SRC, 1, 1, U1><<<grid, 64 * kFewWaves, 0, s>>>(f);
+    else
+        linear_few_kernel<FORMAT, SRC, 2, 1, U2><<<grid, 64 * kFewWaves, 0, s>>>(f);
+    RMR_HIP(hipGetLastError());
+}
+
+template <int FORMAT>
+void launch_few_mx8(const FewArgs& f, bool kept, int type, hipStream_t s) {
+    if (kept)
+        launch_few<FORMAT, kHeld>(f, s);
+    else if (type == RMR_TYPE_F16)
+        launch_few<FORMAT, kFromF16>(f, s);
+    else if (type == RMR_TYPE_BF16)
+        launch_few<FORMAT, kFromBf16>(f, s);
+    else
+        launch_few<FORMAT, kFromF32>(f, s);
+}
+
+template <int FORMAT, int MT, int G, int WM, int WN>
+void launch_tile(LinearArgs a, hipStream_t s) {
+    a.row_tiles = (a.rows + 16 * MT * WM - 1) / (16 * MT * WM);
+    a.col_tiles = (a.groups + G * WN - 1) / (G * WN);
+    const int64_t tiles = a.row_tiles * a.col_tiles;
+    if (tiles > 1 << 22) fail(RMR_ERR_INVALID_ARGUMENT, "linear: %lld tiles in one call", (long long)tiles);
+    linear_tile_kernel<FORMAT, MT, G, WM, WN><<<(unsigned)tiles, 64 * WM * WN, 0, s>>>(a);
+    RMR_HIP(hipGetLastError());
+}
+
+template <int FORMAT>
+void launch_format(const LinearArgs& a, int cus, hipStream_t s) {
+    const int64_t big = ((a.rows + 255) / 256) * ((a.groups + 3) / 4);
+    const int64_t mid = ((a.rows + 127) / 128) * ((a.groups + 1) / 2);
+    if (FORMAT != kMx8Wide && big >= cus / 2 && a.ksteps >= 16) {
+        if constexpr (FORMAT != kMx8Wide) {
+            if (FORMAT == kMx8)
+                launch_tile<FORMAT, 8, 2, 2, 2>(a, s);   // 1590 TFLOP/s on 8192^3, with eight waves 1280 (spills)
+            else
+                launch_tile<FORMAT, 8, 1, 2, 4>(a, s);   // 1330 TFLOP/s on 8192^3, with four waves 1270
+        }
+    } else if (mid >= cus) {
+        launch_tile<FORMAT, 4, 1, 2, 2>(a, s);
+    } else {
+        launch_tile<FORMAT, 2, 1, 2, 2>(a, s);
+    }
+}
+
+}  // namespace
+
+// -------------------------------------------------------------------------------------------------------------- Linear
+
+Linear::Linear(const rmr_linear_cfg& cfg, const void* weight, int weight_type, int64_t ldw, const float* bias, int mem, hipStream_t s)
+    : ctx_(device_ctx(cfg.device)), cfg_(cfg) {
+    DeviceGuard guard(cfg.device);
+    const int n = cfg.out_features, k = cfg.in_features;
+    const bool mx8 = cfg.format == RMR_LINEAR_MX8;
+    ksteps_ = mx8 ? (k + 127) / 128 : (k + 63) / 64;
+    groups_ = (n + 63) / 64;
+    w_.alloc((size_t)groups_ * ksteps_ * kGroupStep);
+    bias_.alloc((size_t)groups_ * 64);
+    zero_.alloc(kStepBytes);
+    RMR_HIP(hipMemsetAsync(bias_.p, 0, bias_.n * sizeof(float), s));
+    RMR_HIP(hipMemsetAsync(zero_.p, 0, zero_.n, s));
+    if (bias)
+        RMR_HIP(hipMemcpyAsync(bias_.p, bias, (size_t)n * sizeof(float), mem == RMR_MEM_DEVICE ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice, s));
+    DevBuf<unsigned char> staged, q, qs;
+    const void* w = weight;
+    if (mem != RMR_MEM_DEVICE) {
+        const size_t row = (size_t)k * type_bytes(weight_type);
+        staged.alloc(row * n);
+        RMR_HIP(hipMemcpy2DAsync(staged.p, row, weight, (size_t)ldw * type_bytes(weight_type), row, n, hipMemcpyHostToDevice, s));
+        w = staged.p, ldw = k;
+    }
+    const int64_t pieces = (int64_t)groups_ * ksteps_ * (kGroupStep / 16);
+    const unsigned grid = (unsigned)((pieces + 255) / 256 < 65536 ? (pieces + 255) / 256 : 65536);
+    if (mx8) {
+        Mx8Rows rows{nullptr, nullptr, mx8_pitch(k), mx8_scale_pitch(k)};
+        q.alloc((size_t)(rows.pitch * n));
+        qs.alloc((size_t)(rows.scale_pitch * n));
+        wscale_.alloc((size_t)groups_ * ((ksteps_ + 3) / 4) * 256);
+        rows.data = q.p, rows.scale = qs.p;
+        RMR_HIP(hipMemsetAsync(qs.p, 0, qs.n, s));
+        launch_quantise_rows(ctx_, s, RowSource{w, weight_type, ldw}, k, n, rows);
+        pack_mx8_kernel<<<grid, 256, 0, s>>>(PackMx8Args{rows, n, ksteps_, groups_, w_.p, wscale_.p});
+    } else {
+        const PackArgs pa{w, ldw, n, k, ksteps_, groups_, w_.p};
+        const bool bf = cfg.format == RMR_LINEAR_BF16;
+        if (weight_type == RMR_TYPE_F16)
+            bf ? pack_weight_kernel<F16, BF16><<<grid, 256, 0, s>>>(pa) : pack_weight_kernel<F16, F16><<<grid, 256, 0, s>>>(pa);
+        else if (weight_type == RMR_TYPE_BF16)
+            bf ? pack_weight_kernel<BF16, BF16><<<grid, 256, 0, s>>>(pa) : pack_weight_kernel<BF16, F16><<<grid, 256, 0, s>>>(pa);
+        else
+            bf ? pack_weight_kernel<float, BF16><<<grid, 256, 0, s>>>(pa) : pack_weight_kernel<float, F16><<<grid, 256, 0, s>>>(pa);
+    }
+    RMR_HIP(hipGetLastError());
+    RMR_HIP(hipStreamSynchronize(s));   // any stream may use the layer from here on, and the caller's weights are free
+}
+
+struct Linear::Plan {
+    size_t x_bytes = 0, scale_bytes = 0;   // staged rows in the workspace: aligned 16-bit rows, or quantised ones
+    size_t total() const { return x_bytes + scale_bytes; }
+};
+
+Linear::Plan Linear::plan(const Call& c) const {
+    Plan p;
+    if (c.rows <= kFewRows || c.kept) return p;
+    if (cfg_.format == RMR_LINEAR_MX8) {
+        p.x_bytes = (size_t)(c.rows * mx8_pitch(cfg_.in_features));
+        p.scale_bytes = (size_t)(c.rows * mx8_scale_pitch(cfg_.in_features));
+    } else if (cfg_.in_features % 8 || (c.ld_bytes() % 16 && c.rows > 1) || (uintptr_t)c.x.p % 16) {
+        p.x_bytes = (size_t)(c.rows * ksteps_ * kStepBytes);
+    }
+    return p;
+}
+
+size_t Linear::workspace_bytes(const Call& c) const { return plan(c).total(); }
+
+void Linear::run(const Call& c) {
+    if (c.rows <= 0) return;
+    const Plan p = plan(c);
+    if (p.total() > c.workspace_bytes || (p.total() && !c.workspace))
+        fail(RMR_ERR_CAPACITY, "linear: the call needs %zu bytes of workspace, %zu given", p.total(), c.workspace_bytes);
+    if (p.total() && (uintptr_t)c.workspace % 16) fail(RMR_ERR_INVALID_ARGUMENT, "linear: the workspace must be 16-byte aligned");
+    DeviceGuard guard(ctx_.device);
+    LinearArgs a{};
+    a.rows = c.rows, a.last_chunks = 8, a.zero = zero_.p;
+    a.w = w_.p, a.w_scale = wscale_.p, a.bias = bias_.p;
+    a.ksteps = ksteps_, a.groups = groups_, a.out_features = cfg_.out_features;
+    a.residual = c.residual, a.ldr = c.ldr, a.y = c.y, a.ldy = c.ldy, a.y_type = c.y_type, a.act = cfg_.activation;
+    if (c.kept) {
+        const Mx8Rows r = c.cache->rows();
+        a.x = r.data, a.x_pitch = r.pitch, a.x_scale = r.scale, a.x_scale_pitch = r.scale_pitch;
+        a.slots = c.slots, a.n_slots = c.cache->slots();
+    } else if (c.rows <= kFewRows) {
+        // read as it is
+    } else if (cfg_.format == RMR_LINEAR_MX8) {
+        const Mx8Rows r{(unsigned char*)c.workspace, (unsigned char*)c.workspace + p.x_bytes, mx8_pitch(cfg_.in_features), mx8_scale_pitch(cfg_.in_features)};
+        launch_quantise_rows(ctx_, c.stream, c.x, cfg_.in_features, c.rows, r);
+        a.x = r.data, a.x_pitch = r.pitch, a.x_scale = r.scale, a.x_scale_pitch = r.scale_pitch;
+    } else if (p.x_bytes) {
+        const AlignArgs al{c.x.p, c.x.ld, c.rows, cfg_.in_features, ksteps_ * 8, (unsigned char*)c.workspace};
+        const int64_t blocks = (c.rows * al.per_row + 255) / 256;
+        align_rows_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, c.stream>>>(al);
+        a.x = (const unsigned char*)c.workspace, a.x_pitch = (int64_t)ksteps_ * kStepBytes;
+    } else {
+        a.x = (const unsigned char*)c.x.p, a.x_pitch = c.ld_bytes();
+        a.last_chunks = (cfg_.in_features - (ksteps_ - 1) * 64) / 8;
+    }
+    const double out = (double)c.rows * cfg_.out_features;
+    ProfScope prof(ctx_.prof, c.stream, "linear", 2.0 * out * cfg_.in_features,
+                   (double)w_.n + (double)c.rows * ksteps_ * kStepBytes + out * type_bytes(c.y_type) * (c.residual ? 2 : 1));
+    if (c.rows <= kFewRows) {
+        const FewArgs f{a, c.x.p, c.x.ld, cfg_.in_features};
+        if (cfg_.format == RMR_LINEAR_F16)
+            launch_few<kF16, kRaw>(f, c.stream);
+        else if (cfg_.format == RMR_LINEAR_BF16)
+            launch_few<kBf16, kRaw>(f, c.stream);
+        else if (c.y_type != RMR_TYPE_F32)
+            launch_few_mx8<kMx8>(f, c.kept, c.x.type, c.stream);
+        else
+            launch_few_mx8<kMx8Wide>(f, c.kept, c.x.type, c.stream);
+        return;
+    }
+    if (cfg_.format == RMR_LINEAR_F16)
+        launch_format<kF16>(a, ctx_.num_cus, c.stream);
+    else if (cfg_.format == RMR_LINEAR_BF16)
+        launch_format<kBf16>(a, ctx_.num_cus, c.stream);
+    else if (c.y_type != RMR_TYPE_F32)
+        launch_format<kMx8>(a, ctx_.num_cus, c.stream);
+    else
+        launch_format<kMx8Wide>(a, ctx_.num_cus, c.stream);
+}
+
+}  // namespace rmr

@@ -54,6 +54,8 @@ class Yolov8 {
     // the last forward(), as f32 [h][w][c] on the host (out = nullptr: the dimensions only).  Needs a detector
     // created with RMR_ARENA_REUSE=0 (otherwise later layers have overwritten the stage outputs).
     bool read_feature(hipStream_t s, const std::string& name, int img, float* out, int dims[3]);
+    // the same stage output where it lies: pixels ld halves apart (a null pointer for an unknown stage)
+    const __half* stage_rows(const std::string& name, int img, int dims[3], int64_t& ld);
 
     // network input: f16 NHWC with 8 channels per pixel (RGB + 5 zero lanes), [max_batch]
     __half* input() { return input_.p; }

@@ -1514,6 +1514,19 @@ bool Yolov8::read_feature(hipStream_t s, const std::string& name, int img, float
     return true;
 }
 
+const __half* Yolov8::stage_rows(const std::string& name, int img, int dims[3], int64_t& ld) {
+    const auto it = named_.find(name);
+    if (it == named_.end()) return nullptr;
+    const View& v = it->second.v;
+    dims[0] = v.h, dims[1] = v.w, dims[2] = v.c;
+    if (img < 0 || img >= chunk_) fail(RMR_ERR_INVALID_ARGUMENT, "stage %s: image %d is outside the last chunk", name.c_str(), img);
+    if (arena_reuse_)
+        fail(RMR_ERR_LOGIC, "stage outputs are overwritten by later layers when the arena is compacted; "
+                            "create the detector with RMR_ARENA_REUSE=0 in the environment");
+    ld = v.cs;
+    return arena_.p + v.off * chunk_ + (size_t)img * v.h * v.w * v.cs + v.co;
+}
+
 Yolov8::~Yolov8() {
     for (auto& kv : graphs_) {
         if (kv.second.exec) (void)hipGraphExecDestroy(kv.second.exec);
