@@ -37,6 +37,15 @@ enum { kF16 = RMR_LINEAR_F16, kBf16 = RMR_LINEAR_BF16, kMx8 = RMR_LINEAR_MX8, kM
 constexpr int kStepBytes = 128;      // of a row, per K step
 constexpr int kGroupStep = 8192;     // bytes of one K step of 64 output features
 
+// f(integral_constant<K>) ... f(integral_constant<N - 1>)
+template <int K, int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (K < N) {
+        f(std::integral_constant<int, K>{});
+        static_for<K + 1, N>(std::forward<F>(f));
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ laying out the weights
 
 // feature of the group of 64 that sits in slot `slot` of operand j
@@ -132,21 +141,20 @@ __global__ __launch_bounds__(256) void align_rows_kernel(AlignArgs a) {
 
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
+    constexpr float kLog2e = 1.44269504f;
     if constexpr (ACT == RMR_ACT_RELU) return v < 0.0f ? 0.0f : v;
-    if constexpr (ACT == RMR_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v));
-    if constexpr (ACT == RMR_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+    if constexpr (ACT == RMR_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
+    if constexpr (ACT == RMR_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
     if constexpr (ACT == RMR_ACT_GELU) {
         // v / 2 erfc(-v / sqrt 2) with Abramowitz & Stegun 7.1.26: erfc(z) = t (a1 + t (a2 + ...)) e^(-z z), t = 1 / (1 + p z), z >= 0,
-        // off by at most 1.5e-7 absolutely, which is 0.75e-7 |v| here
-        const float z = fabsf(v) * 0.70710678f;
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-        float q = fmaf(1.061405429f, t, -1.453152027f);
-        q = fmaf(q, t, 1.421413741f);
-        q = fmaf(q, t, -0.284496736f);
-        q = fmaf(q, t, 0.254829592f);
-        q *= t * __expf(-z * z);                       // erfc(|v| / sqrt 2)
-        const float h = 0.5f * v;
-        return v < 0.0f ? h * q : h * (2.0f - q);
+        // off by at most 1.5e-7 absolutely, which is 0.75e-7 |v| here; the coefficients are halved, z = |v| / sqrt 2
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(v), 1.0f));
+        float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+        q = fmaf(q, t, 0.5f * 1.421413741f);
+        q = fmaf(q, t, 0.5f * -0.284496736f);
+        q = fmaf(q, t, 0.5f * 0.254829592f);
+        q *= t * __builtin_amdgcn_exp2f(-0.5f * kLog2e * (v * v));   // erfc(|v| / sqrt 2) / 2
+        return v * (v < 0.0f ? q : 1.0f - q);
     }
     return v;
 }
@@ -176,65 +184,106 @@ struct LinearArgs {
     int col_tiles;
 };
 
-template <class T>
-__device__ __forceinline__ void store_row(const LinearArgs& a, const f32x4 (&v)[4], int64_t row, int c0, int have) {
-    constexpr int V = 16 / (int)sizeof(T);
-    T* y = (T*)a.y + row * a.ldy + c0;
-    const T* r = a.residual ? (const T*)a.residual + row * a.ldr + c0 : nullptr;
-#pragma unroll
-    for (int p = 0; p < 16 / V; ++p) {
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = v[(p * V + i) >> 2][(p * V + i) & 3];
+// One operand row of the epilogue: 16 features c0 ... c0 + 15 of one row of x, v[j][i] = feature c0 + 4 j + i before the bias.  A wave
+// whose rows and features are all there takes the straight path: residual loads of a batch of rows first, then arithmetic and
+// stores, 16 bytes each.  At the edges of y a lane goes through `spill`, its own 64 bytes of LDS, value by value.
+template <class T, int ACT, int MT, int Q, class Acc>
+__device__ __forceinline__ void finish_full(const LinearArgs& a, Acc&& acc, const f32x4 (&bias)[4], int64_t row0, int c0) {
+    constexpr int V = 16 / (int)sizeof(T), P = 16 / V;   // values of a piece, pieces of 16 features
+    constexpr int B = MT < 4 ? MT : 4;                   // rows of a batch
+    T* y = (T*)a.y + row0 * a.ldy + c0;
+    const T* r = a.residual ? (const T*)a.residual + row0 * a.ldr + c0 : nullptr;
+    const int64_t ystep = 16 * a.ldy, rstep = 16 * a.ldr;
+    static_for<0, MT / B>([&](auto batch) {
+        u32x4 rv[B][P];
         if (r) {
-            float rv[V];
-            load_values<T>(r + p * V, have - p * V, rv);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] += rv[i];
+            for (int m = 0; m < B; ++m) {
+#pragma unroll
+                for (int p = 0; p < P; ++p) rv[m][p] = *(const u32x4_any*)(r + p * V);
+                r += rstep;
+            }
         }
-        store_values<T>(y + p * V, have - p * V, o);
-    }
+        static_for<0, B>([&](auto in) {
+            constexpr int b = decltype(in)::value, m = decltype(batch)::value * B + b;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                union {
+                    u32x4 u;
+                    T t[V];
+                } w;
+                w.u = r ? rv[b][p] : u32x4{0, 0, 0, 0};
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const int k = p * V + i;
+                    o[i] = activate<ACT>(acc(std::integral_constant<int, m>{})[Q * 4 + (k >> 2)][k & 3] + bias[k >> 2][k & 3]);
+                    if (r) o[i] += to_f32(w.t[i]);
+                }
+                store_values<T>(y + p * V, V, o);
+            }
+            y += ystep;
+        });
+    });
 }
 
-template <int ACT>
-__device__ __forceinline__ void activate_row(f32x4 (&v)[4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[j][i] = activate<ACT>(v[j][i]);
-}
-
-// 16 features c0 ... of one row: v[j][i] is feature c0 + 4 j + i before the bias
-__device__ __forceinline__ void finish_row(const LinearArgs& a, f32x4 (&v)[4], const f32x4 (&bias)[4], int64_t row, int c0) {
+template <class T>
+__device__ void finish_edge(const LinearArgs& a, const f32x4 (&v)[4], float* spill, int64_t row, int c0) {
     const int have = a.out_features - c0;
     if (row >= a.rows || have <= 0) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += bias[j];
-    switch (a.act) {
-        case RMR_ACT_RELU: activate_row<RMR_ACT_RELU>(v); break;
-        case RMR_ACT_SILU: activate_row<RMR_ACT_SILU>(v); break;
-        case RMR_ACT_GELU: activate_row<RMR_ACT_GELU>(v); break;
-        case RMR_ACT_SIGMOID: activate_row<RMR_ACT_SIGMOID>(v); break;
-        default: break;
+    for (int j = 0; j < 4; ++j) *(f32x4*)(spill + 4 * j) = v[j];
+    T* y = (T*)a.y + row * a.ldy + c0;
+    const T* r = a.residual ? (const T*)a.residual + row * a.ldr + c0 : nullptr;
+#pragma unroll 1
+    for (int i = 0; i < 16 && i < have; ++i) {
+        float f = spill[i] + a.bias[c0 + i];
+        switch (a.act) {
+            case RMR_ACT_RELU: f = activate<RMR_ACT_RELU>(f); break;
+            case RMR_ACT_SILU: f = activate<RMR_ACT_SILU>(f); break;
+            case RMR_ACT_GELU: f = activate<RMR_ACT_GELU>(f); break;
+            case RMR_ACT_SIGMOID: f = activate<RMR_ACT_SIGMOID>(f); break;
+            default: break;
+        }
+        y[i] = from_f32<T>(f + (r ? to_f32(r[i]) : 0.0f));
     }
+}
+
+// a wave's 16 MT rows x 64 features: operand set Q of acc(m)
+template <class T, int MT, int Q, class Acc>
+__device__ __forceinline__ void finish_typed(const LinearArgs& a, Acc&& acc, float* spill, int64_t row0, int n0, int lane) {
+    const int c0 = n0 + (lane >> 4) * 16;
+    const int64_t row = row0 + (lane & 15);
+    if (row0 + 16 * MT <= a.rows && n0 + 64 <= a.out_features) {
+        f32x4 bias[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = *(const f32x4*)(a.bias + c0 + j * 4);
+        switch (a.act) {
+            case RMR_ACT_RELU: finish_full<T, RMR_ACT_RELU, MT, Q>(a, acc, bias, row, c0); break;
+            case RMR_ACT_SILU: finish_full<T, RMR_ACT_SILU, MT, Q>(a, acc, bias, row, c0); break;
+            case RMR_ACT_GELU: finish_full<T, RMR_ACT_GELU, MT, Q>(a, acc, bias, row, c0); break;
+            case RMR_ACT_SIGMOID: finish_full<T, RMR_ACT_SIGMOID, MT, Q>(a, acc, bias, row, c0); break;
+            default: finish_full<T, RMR_ACT_NONE, MT, Q>(a, acc, bias, row, c0); break;
+        }
+    } else {
+        static_for<0, MT>([&](auto mm) {
+            const f32x4 v[4] = {acc(mm)[Q * 4], acc(mm)[Q * 4 + 1], acc(mm)[Q * 4 + 2], acc(mm)[Q * 4 + 3]};
+            finish_edge<T>(a, v, spill, row + 16 * decltype(mm)::value, c0);
+        });
+    }
+}
+
+template <int MT, int Q, class Acc>
+__device__ __forceinline__ void finish_group(const LinearArgs& a, Acc&& acc, float* spill, int64_t row0, int n0, int lane) {
     if (a.y_type == RMR_TYPE_F16)
-        store_row<F16>(a, v, row, c0, have);
+        finish_typed<F16, MT, Q>(a, acc, spill, row0, n0, lane);
     else if (a.y_type == RMR_TYPE_BF16)
-        store_row<BF16>(a, v, row, c0, have);
+        finish_typed<BF16, MT, Q>(a, acc, spill, row0, n0, lane);
     else
-        store_row<float>(a, v, row, c0, have);
+        finish_typed<float, MT, Q>(a, acc, spill, row0, n0, lane);
 }
 
 // ------------------------------------------------------------------------------------------------------- the tile kernel
-
-// f(integral_constant<K>) ... f(integral_constant<N - 1>)
-template <int K, int N, class F>
-__device__ __forceinline__ void static_for(F&& f) {
-    if constexpr (K < N) {
-        f(std::integral_constant<int, K>{});
-        static_for<K + 1, N>(std::forward<F>(f));
-    }
-}
 
 // 64 lanes x 16 bytes of global memory to LDS at lds + lane * 16 where `mask` is -1, nothing where it is 0 (uniform; the wave's 64
 // lanes are all active here)
@@ -569,19 +618,13 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
         });
     }
 
+    // (the LDS that a lane of an edge tile writes may still be read by a slower wave's last fragment loads, whose values nobody uses)
+    float* spill = (float*)smem + threadIdx.x * 16;
     static_for<0, G>([&](auto group) {
         constexpr int q = decltype(group)::value;
         const int gr = g0 + wn * G + q;
-        if (gr >= a.groups) return;
-        const int c0 = gr * 64 + g * 16;
-        f32x4 bias[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bias[j] = *(const f32x4*)(a.bias + c0 + j * 4);
-        static_for<0, MT>([&](auto mm) {
-            constexpr int m = decltype(mm)::value;
-            f32x4 v[4] = {acc[m][q * 4], acc[m][q * 4 + 1], acc[m][q * 4 + 2], acc[m][q * 4 + 3]};
-            finish_row(a, v, bias, m0 + wm * MT * 16 + m * 16 + (lane & 15), c0);
-        });
+        if (gr < a.groups)
+            finish_group<MT, q>(a, [&](auto m) -> f32x4(&)[J] { return acc[decltype(m)::value]; }, spill, m0 + wm * MT * 16, gr * 64, lane);
     });
 }
 
