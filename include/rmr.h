@@ -471,6 +471,8 @@ typedef struct {
     void* workspace;        /* DEVICE, 16-byte aligned, not shared with a call that may run at the same time */
     size_t workspace_bytes; /* at least rmr_linear_workspace of the same call */
 } rmr_linear_call;
+/* calls of up to so many rows need no workspace */
+#define RMR_LINEAR_FEW_ROWS 32
 /* bytes of workspace that a call with these operands needs (its workspace fields are not read); kept: through rmr_linear_run_kept */
 rmr_status rmr_linear_workspace(const rmr_linear* layer, const rmr_linear_call* call, int kept, size_t* bytes);
 rmr_status rmr_linear_run(rmr_linear* layer, const rmr_linear_call* call, void* stream);

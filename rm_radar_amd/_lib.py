@@ -14,6 +14,7 @@ OK, ERR_INVALID_ARGUMENT, ERR_RUNTIME, ERR_LOGIC, ERR_DEVICE, ERR_CAPACITY = ran
 MEM_HOST, MEM_DEVICE = 0, 1
 FMT_U8_HWC, FMT_F32_NCHW = 0, 1
 MAX_ARMORS = 64
+LINEAR_FEW_ROWS = 32
 
 
 class RmrError(RuntimeError):

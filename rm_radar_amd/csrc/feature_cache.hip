@@ -69,23 +69,19 @@ __global__ __launch_bounds__(kThreads) void quantise_rows_kernel(WriteArgs a) {
             int64_t to = a.first + r0 + r;
             if constexpr (DEST != DEST_RUN) to = later[r] ? -1 : dest[r];
             if (to < 0) continue;   // lanes of one block share their row
-            float v[V];
-            load_values<T>((const T*)a.x + (r0 + r) * a.ld + c, a.width - c, v);
-            float top = 0.0f;
+            const u32x4 x = load_words<T>((const T*)a.x + (r0 + r) * a.ld + c, a.width - c);
+            const unsigned w[4] = {x[0], x[1], x[2], x[3]};
+            unsigned q[V / 4];
+            const int e = quantise_words<T>(w, q, [](unsigned t) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float m = fabsf(v[k]);
-                top = is_finite(m) && m > top ? m : top;
-            }
-#pragma unroll
-            for (int x = 1; x < 32 / V; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-            const int e = mx8_exponent(top);
-            const float inv = mx8_inverse(e);
+                for (int k = 1; k < 32 / V; k *= 2) t = max(t, (unsigned)__shfl_xor((int)t, k));
+                return t;
+            });
             unsigned char* p = a.data + to * a.pitch + c;
             if constexpr (V == 8)
-                *(u32x2*)p = u32x2{to_e4m3x4(v, inv), to_e4m3x4(v + 4, inv)};
+                *(u32x2*)p = u32x2{q[0], q[1]};
             else
-                *(unsigned*)p = to_e4m3x4(v, inv);
+                *(unsigned*)p = q[0];
             if ((c & 31) == 0) a.scale[to * a.scale_pitch + mx8_scale_at(c >> 5)] = (unsigned char)(e + 127);
         }
     }

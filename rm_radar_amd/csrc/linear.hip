@@ -179,14 +179,17 @@ struct LinearArgs {
     void* y;
     int64_t ldy;
     int y_type, act;
-    int wide;   // y and residual move in 16-byte pieces
     int64_t row_tiles;
     int col_tiles;
+    // K split over workgroups: split i multiplies steps [i * split_steps, ...) and leaves its f32 sums in
+    // partial[i][rows][64 groups]; a second launch joins them in order.  0: one workgroup does all of K
+    int split_steps;
+    float* partial;
 };
 
 // One operand row of the epilogue: 16 features c0 ... c0 + 15 of one row of x, v[j][i] = feature c0 + 4 j + i before the bias.  A wave
 // whose rows and features are all there takes the straight path: residual loads of a batch of rows first, then arithmetic and
-// stores, 16 bytes each.  At the edges of y a lane goes through `spill`, its own 64 bytes of LDS, value by value.
+// stores, 16 bytes each.
 template <class T, int ACT, int MT, int Q, class Acc>
 __device__ __forceinline__ void finish_full(const LinearArgs& a, Acc&& acc, const f32x4 (&bias)[4], int64_t row0, int c0) {
     constexpr int V = 16 / (int)sizeof(T), P = 16 / V;   // values of a piece, pieces of 16 features
@@ -227,25 +230,49 @@ __device__ __forceinline__ void finish_full(const LinearArgs& a, Acc&& acc, cons
     });
 }
 
+// a wave at an edge: its MT x 16 values per lane wait in LDS (`spill`, 64 bytes a lane and row, pitch 1024 floats), so that the loop over
+// the rows is one piece of code
 template <class T>
-__device__ void finish_edge(const LinearArgs& a, const f32x4 (&v)[4], float* spill, int64_t row, int c0) {
+__device__ __forceinline__ void finish_edge(const LinearArgs& a, const float* spill, int mt, int64_t row, int c0) {
+    constexpr int V = 16 / (int)sizeof(T);
     const int have = a.out_features - c0;
-    if (row >= a.rows || have <= 0) return;
+    if (have <= 0) return;
+    f32x4 bias[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) *(f32x4*)(spill + 4 * j) = v[j];
-    T* y = (T*)a.y + row * a.ldy + c0;
-    const T* r = a.residual ? (const T*)a.residual + row * a.ldr + c0 : nullptr;
+    for (int j = 0; j < 4; ++j) bias[j] = *(const f32x4*)(a.bias + c0 + j * 4);
 #pragma unroll 1
-    for (int i = 0; i < 16 && i < have; ++i) {
-        float f = spill[i] + a.bias[c0 + i];
-        switch (a.act) {
-            case RMR_ACT_RELU: f = activate<RMR_ACT_RELU>(f); break;
-            case RMR_ACT_SILU: f = activate<RMR_ACT_SILU>(f); break;
-            case RMR_ACT_GELU: f = activate<RMR_ACT_GELU>(f); break;
-            case RMR_ACT_SIGMOID: f = activate<RMR_ACT_SIGMOID>(f); break;
-            default: break;
+    for (int m = 0; m < mt; ++m, row += 16, spill += 1024) {
+        if (row >= a.rows) return;
+        T* y = (T*)a.y + row * a.ldy + c0;
+        float rv[16 / V][V];
+        if (a.residual) {
+            const T* r = (const T*)a.residual + row * a.ldr + c0;
+#pragma unroll
+            for (int p = 0; p < 16 / V; ++p) load_values<T>(r + p * V, have - p * V, rv[p]);
         }
-        y[i] = from_f32<T>(f + (r ? to_f32(r[i]) : 0.0f));
+        float o[16 / V][V];
+        const auto fill = [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 v = *(const f32x4*)(spill + 4 * j) + bias[j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[(4 * j + i) / V][(4 * j + i) % V] = activate<decltype(act)::value>(v[i]);
+            }
+        };
+        switch (a.act) {
+            case RMR_ACT_RELU: fill(std::integral_constant<int, RMR_ACT_RELU>{}); break;
+            case RMR_ACT_SILU: fill(std::integral_constant<int, RMR_ACT_SILU>{}); break;
+            case RMR_ACT_GELU: fill(std::integral_constant<int, RMR_ACT_GELU>{}); break;
+            case RMR_ACT_SIGMOID: fill(std::integral_constant<int, RMR_ACT_SIGMOID>{}); break;
+            default: fill(std::integral_constant<int, RMR_ACT_NONE>{}); break;
+        }
+#pragma unroll
+        for (int p = 0; p < 16 / V; ++p) {
+            if (a.residual)
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[p][i] += rv[p][i];
+            if (have > p * V) store_values<T>(y + p * V, have - p * V, o[p]);
+        }
     }
 }
 
@@ -267,9 +294,10 @@ __device__ __forceinline__ void finish_typed(const LinearArgs& a, Acc&& acc, flo
         }
     } else {
         static_for<0, MT>([&](auto mm) {
-            const f32x4 v[4] = {acc(mm)[Q * 4], acc(mm)[Q * 4 + 1], acc(mm)[Q * 4 + 2], acc(mm)[Q * 4 + 3]};
-            finish_edge<T>(a, v, spill, row + 16 * decltype(mm)::value, c0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *(f32x4*)(spill + decltype(mm)::value * 1024 + 4 * j) = acc(mm)[Q * 4 + j];
         });
+        finish_edge<T>(a, spill, MT, row, c0);
     }
 }
 
@@ -365,13 +393,13 @@ __device__ __forceinline__ int scale_block(int h, int g) {
 
 // One tile of 16 MT WM rows x 64 G WN features; a wave computes 16 MT x 64 G.
 //
-// Two LDS buffers of one K step each.  A step has two (or four) phases, parts of its rows.  While one part multiplies, the next part's
+// NB LDS buffers of one K step each.  A step has two (or four) phases, parts of its rows.  While one part multiplies, the next part's
 // fragments are read from LDS; before the last part every read of the buffer is done, one barrier, and while the last part
-// multiplies the copies of step t + 2 go out into this buffer and the first fragments of step t + 1 come in from the other one.  So
-// a copy has a whole step to land, a fragment a phase, and a step costs one barrier.  Everything that is not a product is dealt
+// multiplies the copies of step t + NB go out into this buffer and the first fragments of step t + 1 come in from the next one.  So
+// a copy has NB - 1 steps to land, a fragment a phase, and a step costs one barrier.  Everything that is not a product is dealt
 // evenly over the products of its phase (sched_barrier keeps it there): the matrix pipe runs while the rest issues in its shadow.
-template <int FORMAT, int MT, int G, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_tile_kernel(LinearArgs a) {
+template <int FORMAT, int MT, int G, int WM, int WN, int NB>
+__global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void linear_tile_kernel(LinearArgs a) {
     constexpr bool kScaled = FORMAT == kMx8 || FORMAT == kMx8Wide;
     constexpr int S = kScales<FORMAT>;
     constexpr int NP = FORMAT == kMx8 && MT == 8 ? 4 : 2;   // phases of a step (four: half the registers for rows)
@@ -382,8 +410,11 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
     constexpr int kWPer = BG * 8 / kWaves;               // copies of 1 KiB of weights per wave and step
     constexpr int kXScale = (BM + 63) / 64 * 1024, kWScale = BG * 1024;   // bytes of four steps' scales
     constexpr int kScalePieces = kXScale / 1024 + BG;
-    static_assert(BM % (8 * kWaves) == 0 && (BG * 8) % kWaves == 0 && MT % NP == 0 && kScalePieces <= 2 * kWaves, "copies divide over the waves");
-    constexpr int kW0 = 2 * kXBytes, kS0 = kW0 + 2 * kWBytes;   // LDS: both buffers' rows, both buffers' weights, two quads of scales
+    constexpr int kScalePer = kScaled ? (kScalePieces + kWaves - 1) / kWaves : 0;
+    constexpr int kCopies = kXPer + kWPer + kScalePer;   // per wave and step; the scales' do something every fourth step
+    static_assert(BM % (8 * kWaves) == 0 && (BG * 8) % kWaves == 0 && MT % NP == 0, "copies divide over the waves");
+    static_assert(NB >= 2 && NB <= 4 && (NB - 1) * kCopies < 64, "the copies in flight fit the counter, the scales two buffers");
+    constexpr int kW0 = NB * kXBytes, kS0 = kW0 + NB * kWBytes;   // LDS: the buffers' rows, their weights, two quads of scales
     __shared__ __attribute__((aligned(1024))) unsigned char smem[kS0 + (kScaled ? 2 * (kXScale + kWScale) : 0)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4;
@@ -402,6 +433,9 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
     }
     const int64_t m0 = mt * BM;
     const int g0 = nt * BG;   // first group of 64 features
+    const int s0 = blockIdx.y * a.split_steps;   // first step (a multiple of 4)
+    const int steps = a.split_steps && a.ksteps - s0 > a.split_steps ? a.split_steps : a.ksteps - s0;
+    const int last_chunks = s0 + steps == a.ksteps ? a.last_chunks : 8;
 
     const auto source_row = [&](int lr, bool& there) {
         int64_t row = m0 + lr;
@@ -423,9 +457,9 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
         const int chunk = (lane & 7) ^ ((lr >> 1) & 7);
         bool there;
         const int64_t row = source_row(lr, there);
-        xp[i] = there ? a.x + row * a.x_pitch + chunk * 16 : a.zero + chunk * 16;
+        xp[i] = there ? a.x + row * a.x_pitch + (int64_t)s0 * kStepBytes + chunk * 16 : a.zero + chunk * 16;
         xinc[i] = there ? kStepBytes : 0;
-        tail |= chunk >= a.last_chunks ? 1u << i : 0u;
+        tail |= chunk >= last_chunks ? 1u << i : 0u;
     }
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
     const unsigned ldsx = __builtin_amdgcn_readfirstlane(lds0 + wave * kXPer * 1024), ldsw = __builtin_amdgcn_readfirstlane(lds0 + kW0 + wave * kWPer * 1024);
@@ -438,9 +472,9 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
     for (int i = 0; i < kWGroups; ++i) {
         int gr = g0 + wave * kWPer / 8 + i;
         if (gr >= a.groups) gr = a.groups - 1;
-        wp[i] = a.w + ((int64_t)gr * a.ksteps * 8 + wave * kWPer % 8) * 1024;
+        wp[i] = a.w + (((int64_t)gr * a.ksteps + s0) * 8 + wave * kWPer % 8) * 1024;
     }
-    // step `t`'s copies go out in order of t: the pointers walk along
+    // the steps' copies go out in order: the pointers walk along.  A step behind the last one copies nothing, but counts.
     const auto copy_x = [&](int i, int buf, int mask) {
         dma_lane(ldsx + buf * kXBytes + i * 1024, xp[i], mask);
         xp[i] += xinc[i];
@@ -450,17 +484,16 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
         if (i % 8 == 7 || i == kWPer - 1) wp[i / 8] += kGroupStep;
     };
     const auto before_copies = [&](int t) {   // the last step of rows that end inside it: what lies behind is read as zero
-        if (t == a.ksteps - 1 && a.last_chunks < 8) {
+        if (t == steps - 1 && last_chunks < 8) {
 #pragma unroll
             for (int i = 0; i < kXPer; ++i)
                 if (tail >> i & 1) xp[i] = a.zero;
         }
     };
-    // four steps' scales: 64 rows' 16 bytes, or a group's 1 KiB, per copy; piece wave + k * kWaves
-    constexpr int kScalePer = kScaled ? (kScalePieces + kWaves - 1) / kWaves : 1;
+    // four steps' scales, with the first of them: 64 rows' 16 bytes, or a group's 1 KiB, per copy; piece wave + k * kWaves
     const int quads = (a.ksteps + 3) / 4;
-    const unsigned char* sp[kScalePer];
-    int sinc[kScalePer];
+    const unsigned char* sp[kScaled ? kScalePer : 1];
+    int sinc[kScaled ? kScalePer : 1];
     if constexpr (kScaled) {
 #pragma unroll
         for (int k = 0; k < kScalePer; ++k) {
@@ -469,23 +502,24 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
                 bool there;
                 const int lr = piece * 64 + lane;
                 const int64_t row = source_row(lr < BM ? lr : BM - 1, there);
-                sp[k] = there ? a.x_scale + row * a.x_scale_pitch : a.zero;
+                sp[k] = there ? a.x_scale + row * a.x_scale_pitch + (s0 >> 2) * 16 : a.zero;
                 sinc[k] = there ? 16 : 0;
             } else {
                 int gr = g0 + piece - kXScale / 1024;
                 if (gr >= a.groups) gr = a.groups - 1;
-                sp[k] = (const unsigned char*)(a.w_scale + (int64_t)gr * quads * 256 + lane * 4);
+                sp[k] = (const unsigned char*)(a.w_scale + ((int64_t)gr * quads + (s0 >> 2)) * 256 + lane * 4);
                 sinc[k] = 1024;
             }
         }
     }
-    const auto copy_scales = [&](int quad, int mask) {
+    const auto copy_scales = [&](int t) {
         if constexpr (kScaled) {
+            const int mask = (t & 3) == 0 && t < steps ? -1 : 0;
 #pragma unroll
             for (int k = 0; k < kScalePer; ++k) {
                 const int piece = wave + k * kWaves;
-                dma_lane(lds0 + kS0 + (quad & 1) * (kXScale + kWScale) + piece * 1024, sp[k], piece < kScalePieces ? mask : 0);
-                sp[k] += mask ? sinc[k] : 0;
+                dma_lane(lds0 + kS0 + ((t >> 2) & 1) * (kXScale + kWScale) + piece * 1024, sp[k], piece < kScalePieces ? mask : 0);
+                sp[k] += mask & sinc[k];
             }
         }
     };
@@ -524,22 +558,22 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
 #pragma unroll
         for (int j = 0; j < J; ++j) acc[m][j] = f32x4{0, 0, 0, 0};
 
-    // ---- the first two steps' copies, the first fragments
-    const auto copy_step = [&](int t, int buf) {
-        before_copies(t);
+    // ---- the first NB steps' copies, the first fragments
 #pragma unroll
-        for (int i = 0; i < kXPer; ++i) copy_x(i, buf, -1);
+    for (int b = 0; b < NB; ++b) {
+        before_copies(b);
+        copy_scales(b);
+        const int mask = b < steps ? -1 : 0;
 #pragma unroll
-        for (int i = 0; i < kWPer; ++i) copy_w(i, buf, -1);
-    };
-    copy_scales(0, -1);
-    copy_step(0, 0);
-    if (a.ksteps > 1) {
-        copy_step(1, 1);
-        asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kXPer + kWPer) : "memory");
-    } else {
-        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        for (int i = 0; i < kXPer; ++i) copy_x(i, b, mask);
+#pragma unroll
+        for (int i = 0; i < kWPer; ++i) copy_w(i, b, mask);
     }
+    // (only copies that surely went out are counted: an empty one need not be)
+    if (steps >= NB)
+        asm volatile("s_waitcnt vmcnt(%0)" : : "n"((NB - 1) * (kXPer + kWPer)) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     asm volatile("s_barrier" : : : "memory");
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -554,9 +588,9 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
     for (int m = 0; m < MH; ++m) read_xs(0, m, m);
 
     // one step an iteration: every accumulator is updated once, and stays in its registers
-    for (int t = 0; t < a.ksteps; ++t) {
+    int buf = 0;
+    for (int t = 0; t < steps; ++t) {
         constexpr int kSlots = MH * J;   // products of a phase, the features outside, the rows inside
-        const int buf = t & 1;
         const int now = kScaled ? scale_at(t) : 0, next = kScaled ? scale_at(t + 1) : 0;
         const auto product = [&](auto phase, auto slot) {
             constexpr int PH = decltype(phase)::value, m = decltype(slot)::value % MH, j = decltype(slot)::value / MH;
@@ -588,11 +622,16 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
             });
         });
         // step t + 1 has landed for every wave, and every wave has read all of step t
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-        const int more = t + 2 < a.ksteps ? -1 : 0;
-        xl0 += buf ? -kXBytes : kXBytes, xl1 += buf ? -kXBytes : kXBytes, wl += buf ? -kWBytes : kWBytes;
-        before_copies(t + 2);
-        copy_scales((t >> 2) + 1, (t & 3) == 1 && (t >> 2) + 1 < quads ? -1 : 0);
+        if (NB > 2 && t + NB <= steps)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((NB - 2) * (kXPer + kWPer)) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+        asm volatile("s_barrier" : : : "memory");
+        const int more = t + NB < steps ? -1 : 0;
+        const bool wrap = buf == NB - 1;
+        xl0 += wrap ? -(NB - 1) * kXBytes : kXBytes, xl1 += wrap ? -(NB - 1) * kXBytes : kXBytes, wl += wrap ? -(NB - 1) * kWBytes : kWBytes;
+        before_copies(t + NB);
+        copy_scales(t + NB);
         // last phase: the next step's first fragments -- a weight fragment right behind the last product of the one it replaces -- and
         // the copies of the step after it
         static_for<0, kSlots>([&](auto slot) {
@@ -604,10 +643,9 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
                 for (int h = 0; h < 2; ++h) wr[s / MH][h] = read_w(s / MH, h);
                 read_ws(next, s / MH);
             }
-            constexpr int kCopies = kXPer + kWPer;
-            static_for<0, kCopies>([&](auto act) {
+            static_for<0, kXPer + kWPer>([&](auto act) {
                 constexpr int i = decltype(act)::value;
-                if constexpr (i * kSlots / kCopies == s) {
+                if constexpr (i * kSlots / (kXPer + kWPer) == s) {
                     if constexpr (i < kXPer)
                         copy_x(i, buf, more);
                     else
@@ -616,10 +654,28 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 ? 1 : 2) void linear_til
             });
             __builtin_amdgcn_sched_barrier(0);
         });
+        buf = wrap ? 0 : buf + 1;
     }
-
+    // (no copy is in flight any more: the last step waited for all of them)
+    if (a.split_steps) {
+        static_for<0, G>([&](auto group) {
+            constexpr int q = decltype(group)::value;
+            const int gr = g0 + wn * G + q;
+            if (gr >= a.groups) return;
+            const int64_t row0 = m0 + wm * MT * 16 + (lane & 15);
+            float* to = a.partial + (((int64_t)blockIdx.y * a.rows + row0) * a.groups + gr) * 64 + g * 16;
+            static_for<0, MT>([&](auto mm) {
+                constexpr int m = decltype(mm)::value;
+                if (row0 + m * 16 < a.rows)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) *(f32x4*)(to + (int64_t)m * 16 * a.groups * 64 + j * 4) = acc[m][q * 4 + j];
+            });
+        });
+        return;
+    }
     // (the LDS that a lane of an edge tile writes may still be read by a slower wave's last fragment loads, whose values nobody uses)
-    float* spill = (float*)smem + threadIdx.x * 16;
+    float* spill = (float*)smem + wave * MT * 1024 + lane * 16;
+    static_assert(kWaves * MT * 4096 <= kS0, "the edge waves' values fit the buffers");
     static_for<0, G>([&](auto group) {
         constexpr int q = decltype(group)::value;
         const int gr = g0 + wn * G + q;
@@ -664,51 +720,16 @@ struct FewArgs {
     int in_features;
 };
 
-// 16 bytes of a row's values, k0 on; zeros behind its end
-template <class T>
-__device__ __forceinline__ u32x4 load_piece(const T* row, int k0, int k) {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (k0 + V <= k) return *(const u32x4_any*)(row + k0);
-    union {
-        u32x4 u;
-        T t[V];
-    } o;
-    o.u = u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (k0 + i < k) o.t[i] = row[k0 + i];
-    return o.u;
-}
-
 // 16 values of a row as e4m3, and their block's exponent byte.  The block's other half is in lane ^ 16.
 template <class T>
 __device__ __forceinline__ u32x4 quantised_chunk(const u32x4 (&raw)[sizeof(T)], unsigned& byte) {
-    constexpr int V = 16 / (int)sizeof(T);
-    float v[16];
+    unsigned w[4 * sizeof(T)], q[4];
 #pragma unroll
-    for (int p = 0; p < (int)sizeof(T); ++p) {
-        union {
-            u32x4 u;
-            T t[V];
-        } o;
-        o.u = raw[p];
+    for (int p = 0; p < (int)sizeof(T); ++p)
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[p * V + i] = to_f32(o.t[i]);
-    }
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float m = fabsf(v[i]);
-        top = is_finite(m) && m > top ? m : top;
-    }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    const int e = mx8_exponent(top);
-    byte = (unsigned)(e + 127);
-    const float inv = mx8_inverse(e);
-    u32x4 q;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = to_e4m3x4(v + 4 * i, inv);
-    return q;
+        for (int i = 0; i < 4; ++i) w[p * 4 + i] = raw[p][i];
+    byte = (unsigned)(quantise_words<T>(w, q, [](unsigned t) { return max(t, (unsigned)__shfl_xor((int)t, 16)); }) + 127);
+    return u32x4{q[0], q[1], q[2], q[3]};
 }
 
 template <class T>
@@ -819,13 +840,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(FewArgs f) {
                 for (int h = 0; h < 2; ++h) {
                     const int chunk = h * 4 + g;
                     if constexpr (SRC == kRaw) {
-                        xv[u][m][h][0] = load_piece<T>(xrow[m], t * 64 + chunk * 8, f.in_features);
+                        xv[u][m][h][0] = load_words<T>(xrow[m] + t * 64 + chunk * 8, f.in_features - (t * 64 + chunk * 8));
                     } else if constexpr (SRC == kHeld) {
                         xv[u][m][h][0] = u32x4{0, 0, 0, 0};
                         if (held[m]) xv[u][m][h][0] = *(const u32x4*)(held[m] + t * kStepBytes + chunk * 16);
                     } else {
 #pragma unroll
-                        for (int p = 0; p < R; ++p) xv[u][m][h][p] = load_piece<T>(xrow[m], t * kStepBytes + chunk * 16 + p * (16 / R), f.in_features);
+                        for (int p = 0; p < R; ++p) {
+                            const int k0 = t * kStepBytes + chunk * 16 + p * (16 / R);
+                            xv[u][m][h][p] = load_words<T>(xrow[m] + k0, f.in_features - k0);
+                        }
                     }
                 }
                 if constexpr (SRC == kHeld)
@@ -887,7 +911,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(FewArgs f) {
 }
 
 // rows up to which the few-rows kernel takes a call
-constexpr int64_t kFewRows = 32;
+constexpr int64_t kFewRows = RMR_LINEAR_FEW_ROWS;
 
 template <int FORMAT, int SRC>
 void launch_few(const FewArgs& f, hipStream_t s) {
@@ -913,31 +937,73 @@ void launch_few_mx8(const FewArgs& f, bool kept, int type, hipStream_t s) {
         launch_few<FORMAT, kFromF32>(f, s);
 }
 
-template <int FORMAT, int MT, int G, int WM, int WN>
-void launch_tile(LinearArgs a, hipStream_t s) {
+// joins the splits' sums, in order, and finishes the rows: four features of one row a thread
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int splits) {
+    const int64_t quads = a.rows * a.groups * 16, stride = a.rows * a.groups * 64;
+    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < quads; p += (int64_t)gridDim.x * 256) {
+        const int64_t row = p / (a.groups * 16);
+        const int c0 = (int)(p - row * (a.groups * 16)) * 4;
+        const float* from = a.partial + p * 4;
+        f32x4 v = *(const f32x4*)from;
+        for (int k = 1; k < splits; ++k) v += *(const f32x4*)(from + k * stride);
+        if (a.y_type == RMR_TYPE_F16)
+            finish_quad<F16>(a, v, row, c0);
+        else if (a.y_type == RMR_TYPE_BF16)
+            finish_quad<BF16>(a, v, row, c0);
+        else
+            finish_quad<float>(a, v, row, c0);
+    }
+}
+
+template <int FORMAT, int MT, int G, int WM, int WN, int NB>
+void launch_tile(LinearArgs a, int splits, hipStream_t s) {
     a.row_tiles = (a.rows + 16 * MT * WM - 1) / (16 * MT * WM);
     a.col_tiles = (a.groups + G * WN - 1) / (G * WN);
     const int64_t tiles = a.row_tiles * a.col_tiles;
     if (tiles > 1 << 22) fail(RMR_ERR_INVALID_ARGUMENT, "linear: %lld tiles in one call", (long long)tiles);
-    linear_tile_kernel<FORMAT, MT, G, WM, WN><<<(unsigned)tiles, 64 * WM * WN, 0, s>>>(a);
+    linear_tile_kernel<FORMAT, MT, G, WM, WN, NB><<<dim3((unsigned)tiles, (unsigned)splits), 64 * WM * WN, 0, s>>>(a);
     RMR_HIP(hipGetLastError());
 }
 
+// what a call of more than kFewRows rows runs: a tile shape and how many workgroups share a tile's K
+enum { kTileBig, kTileMid, kTileSmall };
+struct Choice {
+    int tile, splits, split_steps;
+};
+
+Choice choose(int format, int64_t rows, int groups, int ksteps, int cus) {
+    const int64_t big = ((rows + 255) / 256) * ((groups + 3) / 4);
+    const int64_t mid = ((rows + 127) / 128) * ((groups + 1) / 2);
+    const int64_t small = ((rows + 63) / 64) * ((groups + 1) / 2);
+    Choice c{kTileSmall, 1, 0};
+    if (format != kMx8Wide && big >= cus / 2 && ksteps >= 16)
+        c.tile = kTileBig;
+    else if (mid >= cus)
+        c.tile = kTileMid;
+    if (c.tile == kTileSmall && small < cus) {
+        const int64_t want = 2 * cus / small;
+        int per = (int)((ksteps + want - 1) / want);
+        per = (per + 3) / 4 * 4;   // the scales come by fours
+        if (per < 8) per = 8;
+        if (per < ksteps) c.split_steps = per, c.splits = (ksteps + per - 1) / per;
+    }
+    return c;
+}
+
 template <int FORMAT>
-void launch_format(const LinearArgs& a, int cus, hipStream_t s) {
-    const int64_t big = ((a.rows + 255) / 256) * ((a.groups + 3) / 4);
-    const int64_t mid = ((a.rows + 127) / 128) * ((a.groups + 1) / 2);
-    if (FORMAT != kMx8Wide && big >= cus / 2 && a.ksteps >= 16) {
-        if constexpr (FORMAT != kMx8Wide) {
-            if (FORMAT == kMx8)
-                launch_tile<FORMAT, 8, 2, 2, 2>(a, s);   // 1590 TFLOP/s on 8192^3, with eight waves 1280 (spills)
-            else
-                launch_tile<FORMAT, 8, 1, 2, 4>(a, s);   // 1330 TFLOP/s on 8192^3, with four waves 1270
-        }
-    } else if (mid >= cus) {
-        launch_tile<FORMAT, 4, 1, 2, 2>(a, s);
+void launch_format(LinearArgs a, const Choice& c, hipStream_t s) {
+    a.split_steps = c.split_steps;
+    if (c.tile == kTileBig) {
+        if constexpr (FORMAT != kMx8Wide) launch_tile<FORMAT, 8, 2, 2, 2, 2>(a, 1, s);
+    } else if (c.tile == kTileMid) {
+        launch_tile<FORMAT, 4, 1, 2, 2, 2>(a, 1, s);
     } else {
-        launch_tile<FORMAT, 2, 1, 2, 2>(a, s);
+        launch_tile<FORMAT, 2, 1, 2, 2, 3>(a, c.splits, s);
+        if (c.splits > 1) {
+            const int64_t blocks = (a.rows * a.groups * 16 + 255) / 256;
+            linear_join_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(a, c.splits);
+            RMR_HIP(hipGetLastError());
+        }
     }
 }
 
@@ -994,13 +1060,20 @@ Linear::Linear(const rmr_linear_cfg& cfg, const void* weight, int weight_type, i
 
 struct Linear::Plan {
     size_t x_bytes = 0, scale_bytes = 0;   // staged rows in the workspace: aligned 16-bit rows, or quantised ones
-    size_t total() const { return x_bytes + scale_bytes; }
+    size_t partial_bytes = 0;              // sums of the workgroups that share a tile's K
+    Choice choice{};
+    size_t total() const { return x_bytes + scale_bytes + partial_bytes; }
 };
 
 Linear::Plan Linear::plan(const Call& c) const {
     Plan p;
-    if (c.rows <= kFewRows || c.kept) return p;
-    if (cfg_.format == RMR_LINEAR_MX8) {
+    if (c.rows <= kFewRows) return p;
+    const int format = cfg_.format != RMR_LINEAR_MX8 ? cfg_.format : c.y_type != RMR_TYPE_F32 ? kMx8 : kMx8Wide;
+    p.choice = choose(format, c.rows, groups_, ksteps_, ctx_.num_cus);
+    if (p.choice.splits > 1) p.partial_bytes = (size_t)p.choice.splits * c.rows * groups_ * 64 * sizeof(float);
+    if (c.kept) {
+        // read where they lie
+    } else if (cfg_.format == RMR_LINEAR_MX8) {
         p.x_bytes = (size_t)(c.rows * mx8_pitch(cfg_.in_features));
         p.scale_bytes = (size_t)(c.rows * mx8_scale_pitch(cfg_.in_features));
     } else if (cfg_.in_features % 8 || (c.ld_bytes() % 16 && c.rows > 1) || (uintptr_t)c.x.p % 16) {
@@ -1042,6 +1115,7 @@ void Linear::run(const Call& c) {
         a.x = (const unsigned char*)c.x.p, a.x_pitch = c.ld_bytes();
         a.last_chunks = (cfg_.in_features - (ksteps_ - 1) * 64) / 8;
     }
+    a.partial = (float*)((unsigned char*)c.workspace + p.x_bytes + p.scale_bytes);
     const double out = (double)c.rows * cfg_.out_features;
     ProfScope prof(ctx_.prof, c.stream, "linear", 2.0 * out * cfg_.in_features,
                    (double)w_.n + (double)c.rows * ksteps_ * kStepBytes + out * type_bytes(c.y_type) * (c.residual ? 2 : 1));
@@ -1058,13 +1132,13 @@ void Linear::run(const Call& c) {
         return;
     }
     if (cfg_.format == RMR_LINEAR_F16)
-        launch_format<kF16>(a, ctx_.num_cus, c.stream);
+        launch_format<kF16>(a, p.choice, c.stream);
     else if (cfg_.format == RMR_LINEAR_BF16)
-        launch_format<kBf16>(a, ctx_.num_cus, c.stream);
+        launch_format<kBf16>(a, p.choice, c.stream);
     else if (c.y_type != RMR_TYPE_F32)
-        launch_format<kMx8>(a, ctx_.num_cus, c.stream);
+        launch_format<kMx8>(a, p.choice, c.stream);
     else
-        launch_format<kMx8Wide>(a, ctx_.num_cus, c.stream);
+        launch_format<kMx8Wide>(a, p.choice, c.stream);
 }
 
 }  // namespace rmr

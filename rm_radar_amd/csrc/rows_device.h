@@ -4,6 +4,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 #include "rows.h"
 
 namespace rmr {
@@ -59,6 +61,22 @@ __device__ __forceinline__ void load_values(const T* p, int have, float (&v)[V])
     }
 }
 
+// the same as 4 words
+template <class T>
+__device__ __forceinline__ u32x4 load_words(const T* p, int have) {
+    constexpr int V = 16 / (int)sizeof(T);
+    if (have >= V) return *(const u32x4_any*)p;
+    union {
+        u32x4 u;
+        T t[V];
+    } o;
+    o.u = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < have) o.t[i] = p[i];
+    return o.u;
+}
+
 template <class T, int V = 16 / (int)sizeof(T)>
 __device__ __forceinline__ void store_values(T* p, int have, const float (&v)[V]) {
     union {
@@ -101,6 +119,75 @@ __device__ __forceinline__ unsigned to_e4m3x4(const float* v, float inv) {
     w = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], w, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], w, true);
     return (unsigned)w;
+}
+
+// the magnitude of the largest of some values as f32 bits: monotonic, infinities and NaN above all others
+template <class T, int W>
+__device__ __forceinline__ unsigned words_top(const unsigned (&w)[W]) {
+    if constexpr (sizeof(T) == 4) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) m = max(m, w[i] & 0x7fffffffu);
+        return m;
+    } else {
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        us2 m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < W; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, w[i] & 0x7fff7fffu));
+        const unsigned short t = m[0] > m[1] ? m[0] : m[1];
+        if constexpr (std::is_same_v<T, BF16>) return (unsigned)t << 16;
+        return __float_as_uint((float)__builtin_bit_cast(_Float16, t));
+    }
+}
+
+// W words of a block (all of its values that this lane holds) to e4m3 bytes; exchange(bits) is the maximum over the block's lanes.
+// The usual block costs one packed maximum and half a conversion per value: the scaled conversions divide by 2^e and round once.
+// Blocks with infinities or NaN, and those of e = -127 (their power of two is an f32 subnormal), go value by value.
+template <class T, int W, class Exchange>
+__device__ __forceinline__ int quantise_words(const unsigned (&w)[W], unsigned (&q)[W * (int)sizeof(unsigned) / (int)sizeof(T) / 4], const Exchange& exchange) {
+    constexpr int N = W * 4 / (int)sizeof(T);   // values
+    unsigned top = exchange(words_top<T>(w));
+    const bool odd = top >= 0x7f800000u || (top > 0 && top < 0x08000000u);   // 2^-111 and less: e may be -127
+    if (__builtin_expect(__any(odd), 0)) {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (sizeof(T) == 4)
+                v[i] = __uint_as_float(w[i]);
+            else
+                v[i] = to_f32(T{(unsigned short)(w[i / 2] >> (i & 1) * 16)});
+        }
+        unsigned t = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) t = is_finite(v[i]) ? max(t, __float_as_uint(v[i]) & 0x7fffffffu) : t;
+        top = exchange(t);
+        const int e = mx8_exponent(__uint_as_float(top));
+        const float inv = mx8_inverse(e);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) q[i] = to_e4m3x4(v + 4 * i, inv);
+        return e;
+    }
+    const int e = mx8_exponent(__uint_as_float(top));
+    const float scale = top ? __uint_as_float((unsigned)(e + 127) << 23) : 1.0f;
+    typedef short s2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        s2 d = {0, 0};
+        if constexpr (std::is_same_v<T, F16>) {
+            d = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(d, __builtin_bit_cast(h2, w[2 * i]), scale, false);
+            d = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(d, __builtin_bit_cast(h2, w[2 * i + 1]), scale, true);
+        } else if constexpr (std::is_same_v<T, BF16>) {
+            d = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(d, __builtin_bit_cast(b2, w[2 * i]), scale, false);
+            d = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(d, __builtin_bit_cast(b2, w[2 * i + 1]), scale, true);
+        } else {
+            d = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(d, __uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]), scale, false);
+            d = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(d, __uint_as_float(w[4 * i + 2]), __uint_as_float(w[4 * i + 3]), scale, true);
+        }
+        q[i] = __builtin_bit_cast(unsigned, d);
+    }
+    return e;
 }
 
 }  // namespace rowsdev

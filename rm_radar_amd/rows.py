@@ -14,6 +14,7 @@ from ._lib import InvalidArgument, check, lib
 _FORMATS = {"f16": 0, "bf16": 1, "mx8": 2}
 _ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4}
 _types: dict = {}
+_devices: dict = {}
 
 
 def _torch():
@@ -27,12 +28,18 @@ def _refuse(msg):
     raise InvalidArgument(_lib.ERR_INVALID_ARGUMENT, msg)
 
 
+def _stream(torch, device):
+    """The raw stream torch works on (as an address: no Stream object per call where torch offers that)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _rows(t, what, width, device):
     """A tensor [..., width] as (address, type, row pitch in elements, rows)."""
     kind = _types.get(t.dtype)
     if kind is None:
         _refuse(f"{what}: dtype {t.dtype} is not float16, bfloat16 or float32")
-    if t.device.type != "cuda" or t.device.index != device:
+    if t.get_device() != device:
         _refuse(f"{what} is on {t.device}, not on GPU {device}")
     if t.dim() != 2:
         if t.dim() == 0 or t.shape[-1] != width:
@@ -50,13 +57,25 @@ def _rows(t, what, width, device):
     return t.data_ptr(), kind, pitch, rows
 
 
-def _slots(t, device):
-    torch = _torch()
-    if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+def _slots(torch, t, device):
+    if t.dtype is not torch.int64 or t.dim() != 1 or not t.is_contiguous():
         _refuse("slots must be a packed one-dimensional int64 tensor")
-    if t.device.type != "cuda" or t.device.index != device:
+    if t.get_device() != device:
         _refuse(f"slots are on {t.device}, not on GPU {device}")
     return t.data_ptr(), t.shape[0]
+
+
+def _output(torch, shape, width, dtype, out, device):
+    """The caller's `out` or a new tensor [*shape, width]: (tensor, address, type, row pitch, rows)."""
+    if out is None:
+        kind = _types.get(dtype)
+        if kind is None:
+            _refuse(f"dtype {dtype} is not float16, bfloat16 or float32")
+        out = torch.empty((*shape, width), dtype=dtype, device=_devices.get(device) or _devices.setdefault(device, torch.device("cuda", device)))
+        return out, out.data_ptr(), kind, width, None
+    if dtype is not None and out.dtype != dtype:
+        _refuse(f"out has dtype {out.dtype}, asked for {dtype}")
+    return (out, *_rows(out, "out", width, device))
 
 
 class FeatureCache:
@@ -64,8 +83,8 @@ class FeatureCache:
     an e4m3 step of the block's largest.  A new cache holds zeros."""
 
     def __init__(self, slots, width, device=0):
-        self._h = C.c_void_p()
-        check(lib().rmr_feature_cache_create(device, slots, width, C.byref(self._h)))
+        self._h, self._lib = C.c_void_p(), lib()
+        check(self._lib.rmr_feature_cache_create(device, slots, width, C.byref(self._h)))
         self.slots, self.width, self.device = slots, width, device
 
     def close(self):
@@ -77,30 +96,26 @@ class FeatureCache:
 
     def nbytes(self) -> int:
         """Device memory held."""
-        return lib().rmr_feature_cache_bytes(self._h)
+        return self._lib.rmr_feature_cache_bytes(self._h)
 
     def write(self, x, slots):
         """Row i of x [n, width] enters slot slots[i] (int64 [n] on the GPU).  Rows whose slot does not exist are left out; of
         rows that name one slot the last stays."""
         torch = _torch()
         p, kind, ld, n = _rows(x, "x", self.width, self.device)
-        sp, m = _slots(slots, self.device)
+        sp, m = _slots(torch, slots, self.device)
         if n != m:
             _refuse(f"{n} rows and {m} slots")
-        check(lib().rmr_feature_cache_write(self._h, p, kind, ld, sp, n, torch.cuda.current_stream(self.device).cuda_stream))
+        check(self._lib.rmr_feature_cache_write(self._h, p, kind, ld, sp, n, _stream(torch, self.device)))
 
     def read(self, slots, dtype=None, out=None):
         """The rows in ``slots`` as [n, width] of ``dtype`` (float16 by default) or into ``out``; zeros for slots that do not exist."""
         torch = _torch()
-        sp, n = _slots(slots, self.device)
-        if out is None:
-            out = torch.empty((n, self.width), dtype=dtype or torch.float16, device=slots.device)
-        elif dtype is not None and out.dtype != dtype:
-            _refuse(f"out has dtype {out.dtype}, asked for {dtype}")
-        p, kind, ld, m = _rows(out, "out", self.width, self.device)
-        if n != m:
+        sp, n = _slots(torch, slots, self.device)
+        out, p, kind, ld, m = _output(torch, (n,), self.width, dtype or (torch.float16 if out is None else None), out, self.device)
+        if m is not None and n != m:
             _refuse(f"{n} slots and {m} rows of out")
-        check(lib().rmr_feature_cache_read(self._h, sp, n, p, kind, ld, torch.cuda.current_stream(self.device).cuda_stream))
+        check(self._lib.rmr_feature_cache_read(self._h, sp, n, p, kind, ld, _stream(torch, self.device)))
         return out
 
 
@@ -137,8 +152,8 @@ class Linear:
         cfg = _lib.LinearCfg(device, w.shape[1], w.shape[0], _FORMATS[format], _ACTIVATIONS[activation])
         on_gpu = w.device.type == "cuda"
         stream = torch.cuda.current_stream(device).cuda_stream if on_gpu else None
-        self._h = C.c_void_p()
-        check(lib().rmr_linear_create(C.byref(cfg), w.data_ptr(), _types[w.dtype], w.stride(0), b.data_ptr() if b is not None else None,
+        self._h, self._lib = C.c_void_p(), lib()
+        check(self._lib.rmr_linear_create(C.byref(cfg), w.data_ptr(), _types[w.dtype], w.stride(0), b.data_ptr() if b is not None else None,
                                       _lib.MEM_DEVICE if on_gpu else _lib.MEM_HOST, stream, C.byref(self._h)))
         self.in_features, self.out_features, self.device = w.shape[1], w.shape[0], device
         self.format, self.activation = format, activation
@@ -150,44 +165,40 @@ class Linear:
 
     __del__ = close
 
-    def _run(self, call, lead, residual, out, out_dtype, where, kept):
-        torch = _torch()
-        if out is None:
-            out = torch.empty((*lead, self.out_features), dtype=out_dtype, device=where)
-        elif out_dtype is not None and out.dtype != out_dtype:
-            _refuse(f"out has dtype {out.dtype}, asked for {out_dtype}")
-        call.y, call.y_type, call.ldy, n = _rows(out, "out", self.out_features, self.device)
-        if n != call.rows:
-            _refuse(f"out has {n} rows, the call {call.rows}")
+    def _run(self, torch, x, x_kind, ldx, rows, lead, residual, out, out_dtype, cache, slots):
+        out, p, kind, ldy, n = _output(torch, lead, self.out_features, out_dtype, out, self.device)
+        if n is not None and n != rows:
+            _refuse(f"out has {n} rows, the call {rows}")
+        r, ldr = None, 0
         if residual is not None:
-            call.residual, kind, call.ldr, n = _rows(residual, "residual", self.out_features, self.device)
-            if n != call.rows or kind != call.y_type:
-                _refuse(f"residual has {n} rows of {residual.dtype}, the output {call.rows} of {out.dtype}")
-        need = C.c_size_t()
-        check(lib().rmr_linear_workspace(self._h, C.byref(call), kept is not None, C.byref(need)))
-        if need.value:
-            space = torch.empty(need.value, dtype=torch.uint8, device=where)
-            call.workspace, call.workspace_bytes = space.data_ptr(), need.value
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        if kept is None:
-            check(lib().rmr_linear_run(self._h, C.byref(call), stream))
+            r, r_kind, ldr, n = _rows(residual, "residual", self.out_features, self.device)
+            if n != rows or r_kind != kind:
+                _refuse(f"residual has {n} rows of {residual.dtype}, the output {rows} of {out.dtype}")
+        call = _lib.LinearCall(x, x_kind, ldx, rows, r, ldr, p, kind, ldy)
+        at = C.byref(call)
+        if rows > _lib.LINEAR_FEW_ROWS:
+            need = C.c_size_t()
+            check(self._lib.rmr_linear_workspace(self._h, at, cache is not None, C.byref(need)))
+            if need.value:
+                space = torch.empty(need.value, dtype=torch.uint8, device=out.device)
+                call.workspace, call.workspace_bytes = space.data_ptr(), need.value
+        stream = _stream(torch, self.device)
+        if cache is None:
+            check(self._lib.rmr_linear_run(self._h, at, stream))
         else:
-            check(lib().rmr_linear_run_kept(self._h, kept[0], kept[1], C.byref(call), stream))
+            check(self._lib.rmr_linear_run_kept(self._h, cache, slots, at, stream))
         return out
 
     def __call__(self, x, residual=None, out=None, out_dtype=None):
         """x [..., in_features] -> [..., out_features] of ``out_dtype`` (x's by default), or into ``out``.  ``residual``: like the
         output, may be ``out`` itself."""
-        _torch()
-        call = _lib.LinearCall()
-        call.x, call.x_type, call.ldx, call.rows = _rows(x, "x", self.in_features, self.device)
-        return self._run(call, x.shape[:-1], residual, out, out_dtype or (x.dtype if out is None else None), x.device, None)
+        torch = _torch()
+        p, kind, ld, n = _rows(x, "x", self.in_features, self.device)
+        return self._run(torch, p, kind, ld, n, x.shape[:-1], residual, out, out_dtype or (x.dtype if out is None else None), None, None)
 
     def kept(self, cache, slots, residual=None, out=None, out_dtype=None):
         """The layer on the rows that ``cache`` holds in ``slots`` (int64 [n] on the GPU): [n, out_features] of ``out_dtype`` (float16 by
         default).  "mx8" layers only."""
         torch = _torch()
-        call = _lib.LinearCall()
-        sp, call.rows = _slots(slots, self.device)
-        return self._run(call, slots.shape, residual, out, out_dtype or (torch.float16 if out is None else None), slots.device,
-                         (cache._h, sp))
+        sp, n = _slots(torch, slots, self.device)
+        return self._run(torch, None, 0, 0, n, (n,), residual, out, out_dtype or (torch.float16 if out is None else None), cache._h, sp)

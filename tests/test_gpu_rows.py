@@ -99,6 +99,25 @@ def test_cache_extreme_values(rmr):
     assert (((want - x.double()).abs() <= x.double().abs() * 2.0 ** -4 + torch.clamp(top * 2 / 448, min=2.0 ** -127) * 2.0 ** -10) | ~fin).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("order", ["counted", "mixed", "magnitude"])
+def test_cache_every_16_bit_value(rmr, kind, order):
+    """All 65536 bit patterns, in blocks of neighbours, of anything beside anything, and of neighbours next to one larger value."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16)
+    if order == "mixed":
+        bits = bits[torch.randperm(65536, generator=torch.Generator().manual_seed(9))]
+    x = bits.view(KINDS[kind]).reshape(-1, 32).clone()
+    if order == "magnitude":
+        top = torch.where(torch.isfinite(x), x.abs().float(), torch.zeros(())).amax(1)
+        x[:, 0] = (top * torch.exp2((torch.arange(len(x)) % 12).float())).clamp_max(6e4).to(x.dtype)
+    cache = rmr.FeatureCache(len(x), 32)
+    s = torch.arange(len(x)).cuda()
+    cache.write(x.cuda(), s)
+    got, want = cache.read(s, dtype=torch.float32).cpu(), ref.held(x).float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(7.0, posinf=9.0, neginf=8.0), want.nan_to_num(7.0, posinf=9.0, neginf=8.0))
+
+
 def test_cache_beyond_32_bits(rmr):
     """Slots whose byte offset passes 2^32."""
     slots, width = 1100000, 4096
