@@ -688,8 +688,9 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void 
 //
 // Up to 16 MT rows: the weights' bytes are the work, and every one of them goes from memory straight into the registers it is
 // multiplied from -- no LDS, no barrier until the end.  A workgroup owns 16 JN features; its eight waves deal the K steps among
-// themselves (wave v takes steps v, v + 8, ...), each with kFewUnroll steps' loads in flight, and their sums are joined through LDS
-// in wave order, so the result does not depend on timing.  x is read as it is -- any alignment and length -- and quantised in
+// themselves (wave v takes steps v, v + 8, ...) and their sums are joined through LDS in wave order, so the result does not depend on
+// timing.  One step's loads a wave are in flight: two or four cost registers and so waves, and gained nothing (4096 -> 4096 on one
+// row 7.7 us against 7.6 and 8.0).  x is read as it is -- any alignment and length -- and quantised in
 // registers where the format asks for it: no launch in front, no workspace.
 
 constexpr int kFewWaves = 8;
@@ -781,7 +782,7 @@ __device__ __forceinline__ void finish_quad(const LinearArgs& a, f32x4 v, int64_
         if (i < have) y[i] = from_f32<T>(v[i] + (r ? to_f32(r[i]) : 0.0f));
 }
 
-template <int FORMAT, int SRC, int MT, int JN, int U>
+template <int FORMAT, int SRC, int MT, int JN>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(FewArgs f) {
     const LinearArgs& a = f.a;
     constexpr bool kScaled = FORMAT == kMx8 || FORMAT == kMx8Wide;
@@ -818,76 +819,67 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(FewArgs f) {
 #pragma unroll
         for (int j = 0; j < JN; ++j) acc[m][j] = f32x4{0, 0, 0, 0};
 
-    for (int t0 = wave; t0 < a.ksteps; t0 += kFewWaves * U) {
-        u32x4 wv[U][JN][2];
-        unsigned wsv[U][JN][2];
-        u32x4 xv[U][MT][2][R];
-        unsigned xsv[U][MT][2];
+    for (int t = wave; t < a.ksteps; t += kFewWaves) {
+        u32x4 wv[JN][2], xv[MT][2][R];
+        unsigned wsv[JN][2], xsv[MT][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int t = t0 + u * kFewWaves < a.ksteps ? t0 + u * kFewWaves : a.ksteps - 1;   // behind the end: loaded, not used
+        for (int j = 0; j < JN; ++j) {
 #pragma unroll
-            for (int j = 0; j < JN; ++j) {
+            for (int h = 0; h < 2; ++h) wv[j][h] = *(const u32x4*)(w + (int64_t)t * kGroupStep + (j * 2 + h) * 1024);
+            if constexpr (kScaled)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) wv[u][j][h] = *(const u32x4*)(w + (int64_t)t * kGroupStep + (j * 2 + h) * 1024);
-                if constexpr (kScaled)
-#pragma unroll
-                    for (int h = 0; h < S; ++h) wsv[u][j][h] = wsp[(t >> 2) * 256 + j * 64 + scale_block<FORMAT>(h, g) * 16] >> ((t & 3) * 8);
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int chunk = h * 4 + g;
-                    if constexpr (SRC == kRaw) {
-                        xv[u][m][h][0] = load_words<T>(xrow[m] + t * 64 + chunk * 8, f.in_features - (t * 64 + chunk * 8));
-                    } else if constexpr (SRC == kHeld) {
-                        xv[u][m][h][0] = u32x4{0, 0, 0, 0};
-                        if (held[m]) xv[u][m][h][0] = *(const u32x4*)(held[m] + t * kStepBytes + chunk * 16);
-                    } else {
-#pragma unroll
-                        for (int p = 0; p < R; ++p) {
-                            const int k0 = t * kStepBytes + chunk * 16 + p * (16 / R);
-                            xv[u][m][h][p] = load_words<T>(xrow[m] + k0, f.in_features - k0);
-                        }
-                    }
-                }
-                if constexpr (SRC == kHeld)
-#pragma unroll
-                    for (int h = 0; h < S; ++h)
-                        xsv[u][m][h] = held[m] ? *(const unsigned*)(hscale[m] + (t >> 2) * 16 + scale_block<FORMAT>(h, g) * 4) >> ((t & 3) * 8) : 0u;
-            }
+                for (int h = 0; h < S; ++h) wsv[j][h] = wsp[(t >> 2) * 256 + j * 64 + scale_block<FORMAT>(h, g) * 16] >> ((t & 3) * 8);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (t0 + u * kFewWaves >= a.ksteps) break;
-            Operand<FORMAT> wf[JN];
+        for (int m = 0; m < MT; ++m) {
 #pragma unroll
-            for (int j = 0; j < JN; ++j) wf[j].set(wv[u][j], wsv[u][j]);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                u32x4 v[2];
-                unsigned xs[2] = {0, 0};
-                if constexpr (kQuantise) {
-                    unsigned b[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) v[h] = quantised_chunk<T>(xv[u][m][h], b[h]);
-                    if constexpr (FORMAT == kMx8Wide) {
-                        xs[0] = b[0], xs[1] = b[1];
-                    } else {
-                        // lane group g scales block g, whose two chunks 2 g and 2 g + 1 lie in half g / 2 of groups 2 g % 4 and one more
-                        const unsigned both = __shfl(b[0] | b[1] << 8, (lane & 15) + ((g & 1) << 5));
-                        xs[0] = g >> 1 ? both >> 8 : both & 255;
-                    }
+            for (int h = 0; h < 2; ++h) {
+                const int chunk = h * 4 + g;
+                if constexpr (SRC == kRaw) {
+                    const int k0 = t * 64 + chunk * 8;
+                    xv[m][h][0] = load_words<T>(xrow[m] + k0, f.in_features - k0);
+                } else if constexpr (SRC == kHeld) {
+                    xv[m][h][0] = u32x4{0, 0, 0, 0};
+                    if (held[m]) xv[m][h][0] = *(const u32x4*)(held[m] + t * kStepBytes + chunk * 16);
                 } else {
-                    v[0] = xv[u][m][0][0], v[1] = xv[u][m][1][0];
-                    if constexpr (kScaled) xs[0] = xsv[u][m][0], xs[1] = xsv[u][m][S - 1];
-                }
-                Operand<FORMAT> xf;
-                xf.set(v, xs);
 #pragma unroll
-                for (int j = 0; j < JN; ++j) acc[m][j] = step_product<FORMAT>(wf[j], xf, acc[m][j]);
+                    for (int p = 0; p < R; ++p) {
+                        const int k0 = t * kStepBytes + chunk * 16 + p * (16 / R);
+                        xv[m][h][p] = load_words<T>(xrow[m] + k0, f.in_features - k0);
+                    }
+                }
             }
+            if constexpr (SRC == kHeld)
+#pragma unroll
+                for (int h = 0; h < S; ++h)
+                    xsv[m][h] = held[m] ? *(const unsigned*)(hscale[m] + (t >> 2) * 16 + scale_block<FORMAT>(h, g) * 4) >> ((t & 3) * 8) : 0u;
+        }
+        Operand<FORMAT> wf[JN];
+#pragma unroll
+        for (int j = 0; j < JN; ++j) wf[j].set(wv[j], wsv[j]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            u32x4 v[2];
+            unsigned xs[2] = {0, 0};
+            if constexpr (kQuantise) {
+                unsigned b[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v[h] = quantised_chunk<T>(xv[m][h], b[h]);
+                if constexpr (FORMAT == kMx8Wide) {
+                    xs[0] = b[0], xs[1] = b[1];
+                } else {
+                    // lane group g scales block g, whose two chunks 2 g and 2 g + 1 lie in half g / 2 of groups 2 g % 4 and one more
+                    const unsigned both = __shfl(b[0] | b[1] << 8, (lane & 15) + ((g & 1) << 5));
+                    xs[0] = g >> 1 ? both >> 8 : both & 255;
+                }
+            } else {
+                v[0] = xv[m][0][0], v[1] = xv[m][1][0];
+                if constexpr (kScaled) xs[0] = xsv[m][0], xs[1] = xsv[m][S - 1];
+            }
+            Operand<FORMAT> xf;
+            xf.set(v, xs);
+#pragma unroll
+            for (int j = 0; j < JN; ++j) acc[m][j] = step_product<FORMAT>(wf[j], xf, acc[m][j]);
         }
     }
 #pragma unroll
@@ -914,27 +906,33 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(FewArgs f) {
 constexpr int64_t kFewRows = RMR_LINEAR_FEW_ROWS;
 
 template <int FORMAT, int SRC>
-void launch_few(const FewArgs& f, hipStream_t s) {
-    // steps in flight: what fits the registers without spilling
-    constexpr int U1 = SRC == kFromF32 ? 2 : 4, U2 = SRC == kFromF32 ? 1 : SRC == kFromF16 || SRC == kFromBf16 ? 2 : 4;
-    const unsigned grid = (unsigned)f.a.groups * 4;
-    if (f.a.rows <= 16)
-        linear_few_kernel<FORMAT, SRC, 1, 1, U1><<<grid, 64 * kFewWaves, 0, s>>>(f);
+void launch_few(const FewArgs& f, int cus, hipStream_t s) {
+    // 32 features a workgroup instead of 16 where that still leaves work for half the chip (all of it for more than 16 rows): 8192 -> 8192
+    // bf16 on one row 27 us against 38, 4096 -> 8192 mx8 on 16 rows 9.7 against 15; 4096 -> 1024 on one row 6.5 against 4.4
+    const bool one = f.a.rows <= 16;
+    const bool wide = f.a.groups * 2 >= (one ? cus / 2 : cus);
+    const unsigned grid = (unsigned)f.a.groups * (wide ? 2 : 4);
+    if (one && wide)
+        linear_few_kernel<FORMAT, SRC, 1, 2><<<grid, 64 * kFewWaves, 0, s>>>(f);
+    else if (one)
+        linear_few_kernel<FORMAT, SRC, 1, 1><<<grid, 64 * kFewWaves, 0, s>>>(f);
+    else if (wide)
+        linear_few_kernel<FORMAT, SRC, 2, 2><<<grid, 64 * kFewWaves, 0, s>>>(f);
     else
-        linear_few_kernel<FORMAT, SRC, 2, 1, U2><<<grid, 64 * kFewWaves, 0, s>>>(f);
+        linear_few_kernel<FORMAT, SRC, 2, 1><<<grid, 64 * kFewWaves, 0, s>>>(f);
     RMR_HIP(hipGetLastError());
 }
 
 template <int FORMAT>
-void launch_few_mx8(const FewArgs& f, bool kept, int type, hipStream_t s) {
+void launch_few_mx8(const FewArgs& f, bool kept, int type, int cus, hipStream_t s) {
     if (kept)
-        launch_few<FORMAT, kHeld>(f, s);
+        launch_few<FORMAT, kHeld>(f, cus, s);
     else if (type == RMR_TYPE_F16)
-        launch_few<FORMAT, kFromF16>(f, s);
+        launch_few<FORMAT, kFromF16>(f, cus, s);
     else if (type == RMR_TYPE_BF16)
-        launch_few<FORMAT, kFromBf16>(f, s);
+        launch_few<FORMAT, kFromBf16>(f, cus, s);
     else
-        launch_few<FORMAT, kFromF32>(f, s);
+        launch_few<FORMAT, kFromF32>(f, cus, s);
 }
 
 // joins the splits' sums, in order, and finishes the rows: four features of one row a thread
@@ -980,12 +978,19 @@ Choice choose(int format, int64_t rows, int groups, int ksteps, int cus) {
         c.tile = kTileBig;
     else if (mid >= cus)
         c.tile = kTileMid;
-    if (c.tile == kTileSmall && small < cus) {
-        const int64_t want = 2 * cus / small;
-        int per = (int)((ksteps + want - 1) / want);
-        per = (per + 3) / 4 * 4;   // the scales come by fours
-        if (per < 8) per = 8;
-        if (per < ksteps) c.split_steps = per, c.splits = (ksteps + per - 1) / per;
+    // Few tiles and a long K: workgroups share a tile's steps.  The partial sums travel through memory and cost a launch, about as much as
+    // 16 steps, so only from 32 steps on, at least 8 each, and with no more than 6 MB of sums: 64 x 4096 x 4096 bf16 26 us in one
+    // piece, 19 / 15 / 17 us in 2 / 4 / 8; 256 x 1024 x 4096 (16 steps) 9.7 us in one piece, 17 in two.
+    if (c.tile == kTileSmall && ksteps >= 32) {
+        int64_t splits = cus / small;
+        const int64_t room = (6 << 20) / (rows * groups * 64 * 4), steps = ksteps / 8;
+        if (splits > room) splits = room;
+        if (splits > steps) splits = steps;
+        if (splits > 1) {
+            c.split_steps = (int)((ksteps + splits - 1) / splits + 3) / 4 * 4;   // the scales come by fours
+            c.splits = (ksteps + c.split_steps - 1) / c.split_steps;
+            if (c.splits == 1) c.split_steps = 0;
+        }
     }
     return c;
 }
@@ -1122,13 +1127,13 @@ void Linear::run(const Call& c) {
     if (c.rows <= kFewRows) {
         const FewArgs f{a, c.x.p, c.x.ld, cfg_.in_features};
         if (cfg_.format == RMR_LINEAR_F16)
-            launch_few<kF16, kRaw>(f, c.stream);
+            launch_few<kF16, kRaw>(f, ctx_.num_cus, c.stream);
         else if (cfg_.format == RMR_LINEAR_BF16)
-            launch_few<kBf16, kRaw>(f, c.stream);
+            launch_few<kBf16, kRaw>(f, ctx_.num_cus, c.stream);
         else if (c.y_type != RMR_TYPE_F32)
-            launch_few_mx8<kMx8>(f, c.kept, c.x.type, c.stream);
+            launch_few_mx8<kMx8>(f, c.kept, c.x.type, ctx_.num_cus, c.stream);
         else
-            launch_few_mx8<kMx8Wide>(f, c.kept, c.x.type, c.stream);
+            launch_few_mx8<kMx8Wide>(f, c.kept, c.x.type, ctx_.num_cus, c.stream);
         return;
     }
     if (cfg_.format == RMR_LINEAR_F16)

@@ -78,6 +78,17 @@ __device__ __forceinline__ u32x4 load_words(const T* p, int have) {
 }
 
 template <class T, int V = 16 / (int)sizeof(T)>
+__device__ __forceinline__ u32x4 pack_values(const float (&v)[V]) {
+    union {
+        u32x4 u;
+        T t[V];
+    } w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w.t[i] = from_f32<T>(v[i]);
+    return w.u;
+}
+
+template <class T, int V = 16 / (int)sizeof(T)>
 __device__ __forceinline__ void store_values(T* p, int have, const float (&v)[V]) {
     union {
         u32x4 u;
