@@ -315,20 +315,34 @@ __device__ __forceinline__ void finish_group(const LinearArgs& a, Acc&& acc, flo
 
 // 64 lanes x 16 bytes of global memory to LDS at lds + lane * 16 where `mask` is -1, nothing where it is 0 (uniform; the wave's 64
 // lanes are all active here)
+__device__ __forceinline__ uint64_t lanes_of(int mask) {
+    const unsigned m = (unsigned)__builtin_amdgcn_readfirstlane(mask);
+    return (uint64_t)m << 32 | m;
+}
 __device__ __forceinline__ void dma_lane(unsigned lds, const unsigned char* p, int mask) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b64 exec, -1"
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b64 exec, -1"
                  :
-                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p), "s"(__builtin_amdgcn_readfirstlane(mask))
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p), "s"(lanes_of(mask))
                  : "memory");
 }
-// the same from a uniform address + lane offset
-__device__ __forceinline__ void dma_uniform(unsigned lds, const unsigned char* base, unsigned off, int mask) {
+// two KiB in a row: an instruction's offset counts on both sides, so the second address is given 1024 less
+__device__ __forceinline__ void dma_lane_pair(unsigned lds, const unsigned char* p, const unsigned char* q, int mask) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %1, off\n\tglobal_load_lds_dwordx4 %2, off offset:1024\n\ts_mov_b64 exec, -1"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p), "v"(q), "s"(lanes_of(mask))
+        : "memory");
+}
+// the same from a uniform address + lane offset, OFFSET bytes further on both sides
+template <int OFFSET>
+__device__ __forceinline__ void dma_uniform_pair(unsigned lds, const unsigned char* base, unsigned off, int mask) {
     const uint64_t b = (uint64_t)base;
     const uint64_t u = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(b >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((unsigned)b);
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
-                 :
-                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(u), "s"(__builtin_amdgcn_readfirstlane(mask))
-                 : "memory");
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4\n\tglobal_load_lds_dwordx4 %1, %2 offset:%5\n\ts_mov_b64 exec, -1"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(u), "s"(lanes_of(mask)), "n"(OFFSET), "n"(OFFSET + 1024)
+        : "memory");
 }
 
 // 16 e4m3 values times 2^(byte - 127) as two bf16 operands, values 0 ... 7 and 8 ... 15
@@ -457,37 +471,38 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void 
         const int chunk = (lane & 7) ^ ((lr >> 1) & 7);
         bool there;
         const int64_t row = source_row(lr, there);
-        xp[i] = there ? a.x + row * a.x_pitch + (int64_t)s0 * kStepBytes + chunk * 16 : a.zero + chunk * 16;
+        xp[i] = (there ? a.x + row * a.x_pitch + (int64_t)s0 * kStepBytes + chunk * 16 : a.zero + chunk * 16) - (i & 1) * 1024;
         xinc[i] = there ? kStepBytes : 0;
         tail |= chunk >= last_chunks ? 1u << i : 0u;
     }
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
     const unsigned ldsx = __builtin_amdgcn_readfirstlane(lds0 + wave * kXPer * 1024), ldsw = __builtin_amdgcn_readfirstlane(lds0 + kW0 + wave * kWPer * 1024);
     const unsigned woff = lane * 16;
-    // a wave's pieces of 1 KiB of weights: a run of kWPer, inside one group or whole groups
-    static_assert(kWPer % 8 == 0 || 8 % kWPer == 0, "a wave's weight pieces do not straddle groups unevenly");
-    constexpr int kWGroups = (kWPer + 7) / 8;
-    const unsigned char* wp[kWGroups];
-#pragma unroll
-    for (int i = 0; i < kWGroups; ++i) {
-        int gr = g0 + wave * kWPer / 8 + i;
+    // a wave's pieces of 1 KiB of weights: a run of kWPer, inside one group
+    static_assert(kXPer % 2 == 0 && kWPer % 2 == 0 && 8 % kWPer == 0, "the copies go out in pairs, a wave's weight pieces lie in one group");
+    const unsigned char* wp;
+    {
+        int gr = g0 + wave * kWPer / 8;
         if (gr >= a.groups) gr = a.groups - 1;
-        wp[i] = a.w + (((int64_t)gr * a.ksteps + s0) * 8 + wave * kWPer % 8) * 1024;
+        wp = a.w + (((int64_t)gr * a.ksteps + s0) * 8 + wave * kWPer % 8) * 1024;
     }
-    // the steps' copies go out in order: the pointers walk along.  A step behind the last one copies nothing, but counts.
-    const auto copy_x = [&](int i, int buf, int mask) {
-        dma_lane(ldsx + buf * kXBytes + i * 1024, xp[i], mask);
-        xp[i] += xinc[i];
+    // the steps' copies go out in order: the pointers walk along.  A step behind the last one copies nothing.
+    const auto copy_x = [&](auto pair, int buf, int mask) {
+        constexpr int i = decltype(pair)::value * 2;
+        dma_lane_pair(ldsx + buf * kXBytes + i * 1024, xp[i], xp[i + 1], mask);
+        xp[i] += xinc[i], xp[i + 1] += xinc[i + 1];
     };
-    const auto copy_w = [&](int i, int buf, int mask) {
-        dma_uniform(ldsw + buf * kWBytes + i * 1024, wp[i / 8] + (i % 8) * 1024, woff, mask);
-        if (i % 8 == 7 || i == kWPer - 1) wp[i / 8] += kGroupStep;
+    const auto copy_w = [&](auto pair, int buf, int mask) {   // (an offset reaches 4095: two pairs from one address)
+        constexpr int i = decltype(pair)::value * 2;
+        dma_uniform_pair<i % 4 * 1024>(ldsw + buf * kWBytes + i / 4 * 4096, wp + i / 4 * 4096, woff, mask);
+        if (i + 2 == kWPer) wp += kGroupStep;
     };
     const auto before_copies = [&](int t) {   // the last step of rows that end inside it: what lies behind is read as zero
-        if (t == steps - 1 && last_chunks < 8) {
+        // (held rows are padded; and without this branch the loop is one block, in which the products stay where they are put)
+        if (!kScaled && t == steps - 1 && last_chunks < 8) {
 #pragma unroll
             for (int i = 0; i < kXPer; ++i)
-                if (tail >> i & 1) xp[i] = a.zero;
+                if (tail >> i & 1) xp[i] = a.zero - (i & 1) * 1024;
         }
     };
     // four steps' scales, with the first of them: 64 rows' 16 bytes, or a group's 1 KiB, per copy; piece wave + k * kWaves
@@ -564,10 +579,8 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void 
         before_copies(b);
         copy_scales(b);
         const int mask = b < steps ? -1 : 0;
-#pragma unroll
-        for (int i = 0; i < kXPer; ++i) copy_x(i, b, mask);
-#pragma unroll
-        for (int i = 0; i < kWPer; ++i) copy_w(i, b, mask);
+        static_for<0, kXPer / 2>([&](auto pair) { copy_x(pair, b, mask); });
+        static_for<0, kWPer / 2>([&](auto pair) { copy_w(pair, b, mask); });
     }
     // (only copies that surely went out are counted: an empty one need not be)
     if (steps >= NB)
@@ -643,13 +656,13 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void 
                 for (int h = 0; h < 2; ++h) wr[s / MH][h] = read_w(s / MH, h);
                 read_ws(next, s / MH);
             }
-            static_for<0, kXPer + kWPer>([&](auto act) {
+            static_for<0, (kXPer + kWPer) / 2>([&](auto act) {
                 constexpr int i = decltype(act)::value;
-                if constexpr (i * kSlots / (kXPer + kWPer) == s) {
-                    if constexpr (i < kXPer)
-                        copy_x(i, buf, more);
+                if constexpr (i * kSlots / ((kXPer + kWPer) / 2) == s) {
+                    if constexpr (i < kXPer / 2)
+                        copy_x(std::integral_constant<int, i>{}, buf, more);
                     else
-                        copy_w(i - kXPer, buf, more);
+                        copy_w(std::integral_constant<int, i - kXPer / 2>{}, buf, more);
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
