@@ -190,8 +190,8 @@ struct LinearArgs {
 // One operand row of the epilogue: 16 features c0 ... c0 + 15 of one row of x, v[j][i] = feature c0 + 4 j + i before the bias.  A wave
 // whose rows and features are all there takes the straight path: residual loads of a batch of rows first, then arithmetic and
 // stores, 16 bytes each.
-template <class T, int ACT, int MT, int Q, class Acc>
-__device__ __forceinline__ void finish_full(const LinearArgs& a, Acc&& acc, const f32x4 (&bias)[4], int64_t row0, int c0) {
+template <class T, int ACT, int MT, int Q, bool PRE, class Acc>
+__device__ __forceinline__ void finish_full(const LinearArgs& a, Acc&& acc, const u32x4 (&pre)[PRE ? MT : 1][4], const f32x4 (&bias)[4], int64_t row0, int c0) {
     constexpr int V = 16 / (int)sizeof(T), P = 16 / V;   // values of a piece, pieces of 16 features
     constexpr int B = MT < 4 ? MT : 4;                   // rows of a batch
     T* y = (T*)a.y + row0 * a.ldy + c0;
@@ -199,7 +199,12 @@ __device__ __forceinline__ void finish_full(const LinearArgs& a, Acc&& acc, cons
     const int64_t ystep = 16 * a.ldy, rstep = 16 * a.ldr;
     static_for<0, MT / B>([&](auto batch) {
         u32x4 rv[B][P];
-        if (r) {
+        if constexpr (PRE) {
+#pragma unroll
+            for (int m = 0; m < B; ++m)
+#pragma unroll
+                for (int p = 0; p < P; ++p) rv[m][p] = pre[decltype(batch)::value * B + m][p];
+        } else if (r) {
 #pragma unroll
             for (int m = 0; m < B; ++m) {
 #pragma unroll
@@ -277,20 +282,25 @@ __device__ __forceinline__ void finish_edge(const LinearArgs& a, const float* sp
 }
 
 // a wave's 16 MT rows x 64 features: operand set Q of acc(m)
-template <class T, int MT, int Q, class Acc>
-__device__ __forceinline__ void finish_typed(const LinearArgs& a, Acc&& acc, float* spill, int64_t row0, int n0, int lane) {
+template <int MT>
+__device__ __forceinline__ bool all_there(const LinearArgs& a, int64_t row0, int n0) {
+    return row0 + 16 * MT <= a.rows && n0 + 64 <= a.out_features;
+}
+
+template <class T, int MT, int Q, bool PRE, class Acc>
+__device__ __forceinline__ void finish_typed(const LinearArgs& a, Acc&& acc, const u32x4 (&pre)[PRE ? MT : 1][4], float* spill, int64_t row0, int n0, int lane) {
     const int c0 = n0 + (lane >> 4) * 16;
     const int64_t row = row0 + (lane & 15);
-    if (row0 + 16 * MT <= a.rows && n0 + 64 <= a.out_features) {
+    if (all_there<MT>(a, row0, n0)) {
         f32x4 bias[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) bias[j] = *(const f32x4*)(a.bias + c0 + j * 4);
         switch (a.act) {
-            case RMR_ACT_RELU: finish_full<T, RMR_ACT_RELU, MT, Q>(a, acc, bias, row, c0); break;
-            case RMR_ACT_SILU: finish_full<T, RMR_ACT_SILU, MT, Q>(a, acc, bias, row, c0); break;
-            case RMR_ACT_GELU: finish_full<T, RMR_ACT_GELU, MT, Q>(a, acc, bias, row, c0); break;
-            case RMR_ACT_SIGMOID: finish_full<T, RMR_ACT_SIGMOID, MT, Q>(a, acc, bias, row, c0); break;
-            default: finish_full<T, RMR_ACT_NONE, MT, Q>(a, acc, bias, row, c0); break;
+            case RMR_ACT_RELU: finish_full<T, RMR_ACT_RELU, MT, Q, PRE>(a, acc, pre, bias, row, c0); break;
+            case RMR_ACT_SILU: finish_full<T, RMR_ACT_SILU, MT, Q, PRE>(a, acc, pre, bias, row, c0); break;
+            case RMR_ACT_GELU: finish_full<T, RMR_ACT_GELU, MT, Q, PRE>(a, acc, pre, bias, row, c0); break;
+            case RMR_ACT_SIGMOID: finish_full<T, RMR_ACT_SIGMOID, MT, Q, PRE>(a, acc, pre, bias, row, c0); break;
+            default: finish_full<T, RMR_ACT_NONE, MT, Q, PRE>(a, acc, pre, bias, row, c0); break;
         }
     } else {
         static_for<0, MT>([&](auto mm) {
@@ -301,14 +311,14 @@ __device__ __forceinline__ void finish_typed(const LinearArgs& a, Acc&& acc, flo
     }
 }
 
-template <int MT, int Q, class Acc>
-__device__ __forceinline__ void finish_group(const LinearArgs& a, Acc&& acc, float* spill, int64_t row0, int n0, int lane) {
+template <int MT, int Q, bool PRE, class Acc>
+__device__ __forceinline__ void finish_group(const LinearArgs& a, Acc&& acc, const u32x4 (&pre)[PRE ? MT : 1][4], float* spill, int64_t row0, int n0, int lane) {
     if (a.y_type == RMR_TYPE_F16)
-        finish_typed<F16, MT, Q>(a, acc, spill, row0, n0, lane);
+        finish_typed<F16, MT, Q, PRE>(a, acc, pre, spill, row0, n0, lane);
     else if (a.y_type == RMR_TYPE_BF16)
-        finish_typed<BF16, MT, Q>(a, acc, spill, row0, n0, lane);
+        finish_typed<BF16, MT, Q, PRE>(a, acc, pre, spill, row0, n0, lane);
     else
-        finish_typed<float, MT, Q>(a, acc, spill, row0, n0, lane);
+        finish_typed<float, MT, Q, PRE>(a, acc, pre, spill, row0, n0, lane);
 }
 
 // ------------------------------------------------------------------------------------------------------- the tile kernel
@@ -582,7 +592,28 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void 
         static_for<0, kXPer / 2>([&](auto pair) { copy_x(pair, b, mask); });
         static_for<0, kWPer / 2>([&](auto pair) { copy_w(pair, b, mask); });
     }
-    // (only copies that surely went out are counted: an empty one need not be)
+    // A small tile has registers to spare: its residual comes in while it multiplies, and waits there.  (102400 x 384 x 384 with a
+    // residual: see the table of tile shapes below.)
+    constexpr bool kPre = MT * G <= (FORMAT == kMx8Wide ? 2 : 4);
+    u32x4 pre[kPre ? MT : 1][4];
+    if constexpr (kPre) {
+        const int64_t row0 = m0 + wm * MT * 16;
+        const int n0 = (g0 + wn) * 64;
+        if (a.residual && !a.split_steps && all_there<MT>(a, row0, n0)) {
+            const int size = a.y_type == RMR_TYPE_F32 ? 4 : 2;
+            const unsigned char* r = (const unsigned char*)a.residual + ((row0 + (lane & 15)) * a.ldr + n0 + g * 16) * size;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p) pre[m][p] = *(const u32x4_any*)(r + p * 16);
+                if (size == 4)
+#pragma unroll
+                    for (int p = 2; p < 4; ++p) pre[m][p] = *(const u32x4_any*)(r + p * 16);
+                r += 16 * a.ldr * size;
+            }
+        }
+    }
+    // (only copies that surely went out are counted: an empty one need not be, and the residual's loads only make the waits stricter)
     if (steps >= NB)
         asm volatile("s_waitcnt vmcnt(%0)" : : "n"((NB - 1) * (kXPer + kWPer)) : "memory");
     else
@@ -693,7 +724,7 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void 
         constexpr int q = decltype(group)::value;
         const int gr = g0 + wn * G + q;
         if (gr < a.groups)
-            finish_group<MT, q>(a, [&](auto m) -> f32x4(&)[J] { return acc[decltype(m)::value]; }, spill, m0 + wm * MT * 16, gr * 64, lane);
+            finish_group<MT, q, kPre>(a, [&](auto m) -> f32x4(&)[J] { return acc[decltype(m)::value]; }, pre, spill, m0 + wm * MT * 16, gr * 64, lane);
     });
 }
 
