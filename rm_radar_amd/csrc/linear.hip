@@ -592,8 +592,7 @@ __global__ __launch_bounds__(64 * WM * WN, MT * G >= 16 || NB > 3 ? 1 : 2) void 
         static_for<0, kXPer / 2>([&](auto pair) { copy_x(pair, b, mask); });
         static_for<0, kWPer / 2>([&](auto pair) { copy_w(pair, b, mask); });
     }
-    // A small tile has registers to spare: its residual comes in while it multiplies, and waits there.  (102400 x 384 x 384 with a
-    // residual: see the table of tile shapes below.)
+    // A small tile has registers to spare: its residual comes in while it multiplies, and waits there.
     constexpr bool kPre = MT * G <= (FORMAT == kMx8Wide ? 2 : 4);
     u32x4 pre[kPre ? MT : 1][4];
     if constexpr (kPre) {
@@ -1013,19 +1012,33 @@ struct Choice {
     int tile, splits, split_steps;
 };
 
+// Time of a call in us from what the shapes were measured at: a round of tiles costs its steps and what a tile has besides (first
+// copies, epilogue).  A CU holds one big tile or two of the others; one alone runs faster than two together.
+//   us a step (bf16 8192^3 and 64 x 4096 x 4096)   big 1.52   mid 1.0, alone 0.64   small 0.62, alone 0.36
+//   us besides (8192 x 512 x 8192, 4096 x 1024^2)  big 8      mid 4                 small 3
+// 2048 x 4096^2 bf16: big 80, mid 63, small 82; 1000 x 4096^2: 81, 46, 43; 102400 x 384^2 f16: 69, 60, 75; 8192 x 512 x 8192: 82, 87, 101.
+// The mx8 steps (twice the values) differ from these by less than the shapes do.
+double tile_time(int64_t tiles, int ksteps, int cus, int per_cu, double step, double alone, double besides) {
+    const int64_t full = tiles / (per_cu * (int64_t)cus), rest = tiles % (per_cu * (int64_t)cus);
+    return full * (ksteps * step + besides) + (rest > cus ? ksteps * step + besides : rest ? ksteps * alone + besides : 0.0);
+}
+
 Choice choose(int format, int64_t rows, int groups, int ksteps, int cus) {
     const int64_t big = ((rows + 255) / 256) * ((groups + 3) / 4);
     const int64_t mid = ((rows + 127) / 128) * ((groups + 1) / 2);
     const int64_t small = ((rows + 63) / 64) * ((groups + 1) / 2);
     Choice c{kTileSmall, 1, 0};
-    if (format != kMx8Wide && big >= cus / 2 && ksteps >= 16)
-        c.tile = kTileBig;
-    else if (mid >= cus)
+    const double t_small = tile_time(small, ksteps, cus, 2, 0.62, 0.36, 3), t_mid = tile_time(mid, ksteps, cus, 2, 1.0, 0.64, 4);
+    const double t_big = format == kMx8Wide ? 1e30 : tile_time(big, ksteps, cus, 1, 1.52, 1.52, 8);
+    if (t_mid <= t_small && t_mid <= t_big)
         c.tile = kTileMid;
+    else if (t_big < t_small)
+        c.tile = kTileBig;
     // Few tiles and a long K: workgroups share a tile's steps.  The partial sums travel through memory and cost a launch, about as much as
     // 16 steps, so only from 32 steps on, at least 8 each, and with no more than 6 MB of sums: 64 x 4096 x 4096 bf16 26 us in one
     // piece, 19 / 15 / 17 us in 2 / 4 / 8; 256 x 1024 x 4096 (16 steps) 9.7 us in one piece, 17 in two.
-    if (c.tile == kTileSmall && ksteps >= 32) {
+    if (small <= cus / 2 && ksteps >= 32) {
+        c.tile = kTileSmall;
         int64_t splits = cus / small;
         const int64_t room = (6 << 20) / (rows * groups * 64 * 4), steps = ksteps / 8;
         if (splits > room) splits = room;
