@@ -412,7 +412,8 @@ rmr_status rmr_upload_wait(rmr_upload* up, int slot);
  * No reference counterpart: dense operators for what a program does with the detector's features behind the detector -- keep
  * them over frames, run one more head on them.  All tensors are DEVICE memory of the handle's device; calls are enqueued on
  * `stream` (a hipStream_t, NULL = the default stream) and return at once; they allocate nothing and can be captured into a
- * HIP graph.  Rows may start at any multiple of their element size and be any number of elements apart. */
+ * HIP graph.  Rows may start at any multiple of their element size and be any number of elements apart.  One layer may be run
+ * by any number of threads and streams at once. */
 
 enum { RMR_TYPE_F16 = 0, RMR_TYPE_BF16 = 1, RMR_TYPE_F32 = 2 };
 
@@ -434,11 +435,14 @@ rmr_status rmr_feature_cache_write(rmr_feature_cache* cache, const void* x, int 
 rmr_status rmr_feature_cache_read(rmr_feature_cache* cache, const int64_t* slots, int64_t n, void* out, int type, int64_t ld,
                                   void* stream);
 /* The output of backbone / neck stage `name` for image `img` of the detector's last call (rmr_detector_read_feature, under the
- * same conditions) enters the cache without leaving the device: pixel (y, x) in slot first_slot + y * w + x.  Complete on return. */
+ * same conditions) enters the cache without leaving the device: pixel (y, x) in slot first_slot + y * w + x.  Waits for the
+ * device's work in flight first; complete on return.  The call must have been of at most rmr_detector_chunk images. */
 rmr_status rmr_detector_keep_feature(rmr_detector* det, const char* name, int img, rmr_feature_cache* cache, int64_t first_slot);
 
 /* y[i] = act(W x[i] + bias) + residual[i] in one launch, accumulated in f32 and rounded once.
- * F16 / BF16: x and W of that type.  MX8: x and W held as a feature cache holds its rows, x quantised within the call. */
+ * F16 / BF16: x and W of that type.  MX8: x and W held as a feature cache holds its rows, x quantised within the call; a 16-bit y
+ * comes from the block-scaled matrix instructions, whose sums are good to about 2^-13 of the largest product, an f32 y from
+ * products and sums in full f32, at half the rate. */
 enum { RMR_LINEAR_F16 = 0, RMR_LINEAR_BF16 = 1, RMR_LINEAR_MX8 = 2 };
 enum { RMR_ACT_NONE = 0, RMR_ACT_RELU = 1, RMR_ACT_SILU = 2, RMR_ACT_GELU = 3 /* v / 2 erfc(-v / sqrt 2) */, RMR_ACT_SIGMOID = 4 };
 typedef struct {
@@ -454,7 +458,7 @@ typedef struct rmr_linear rmr_linear;
 rmr_status rmr_linear_create(const rmr_linear_cfg* cfg, const void* weight, int weight_type, int64_t ldw, const float* bias, int mem,
                              void* stream, rmr_linear** out);
 void rmr_linear_destroy(rmr_linear* layer);
-/* One call's operands.  x: `rows` rows of x_type, ldx elements apart (F16 / BF16: the layer's type; MX8: any).  y, and residual
+/* One call's operands.  x: `rows` (below 2^31) rows of x_type, ldx elements apart (F16 / BF16: the layer's type; MX8: any).  y, and residual
  * if not NULL: rows of y_type, ldy / ldr elements apart.  residual may BE y (same address and ldr = ldy); apart from that y
  * overlaps no operand, and its rows do not overlap (ldy >= out_features).  Rows are x, or -- rmr_linear_run_kept, MX8
  * layers -- the rows of a cache of width in_features in slots[0 .. rows) (DEVICE array; zeros where there is no such slot). */

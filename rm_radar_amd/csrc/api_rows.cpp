@@ -1,4 +1,6 @@
 // api_rows.cpp -- C-ABI entry points (include/rmr.h) of the feature cache and the linear layer.
+#include <utility>
+
 #include "api_handles.h"
 #include "rows.h"
 
@@ -34,6 +36,19 @@ void check_slots(const char* who, const int64_t* slots, int64_t n) {
     if (n > 0 && (!slots || (uintptr_t)slots % 8)) fail(RMR_ERR_INVALID_ARGUMENT, "%s: slots is null or not aligned", who);
 }
 
+// what is written must leave the slots alone
+void check_apart(const char* who, const Range& written, const int64_t* slots, int64_t n) {
+    if (written.meets(Range(slots, 1, n * 4, 0, RMR_TYPE_F16))) fail(RMR_ERR_INVALID_ARGUMENT, "%s: the output overlaps slots", who);
+}
+
+// a handle that could not be made leaves no error behind for the next launch to report
+template <class F>
+rmr_status guarded_create(F&& f) {
+    const rmr_status s = guarded(std::forward<F>(f));
+    if (s != RMR_OK) (void)hipGetLastError();
+    return s;
+}
+
 Linear::Call call_of(const char* who, const rmr_linear* layer, const rmr_linear_call* c, bool kept) {
     if (!layer || !c) fail(RMR_ERR_INVALID_ARGUMENT, "%s: null argument", who);
     const rmr_linear_cfg& cfg = layer->impl.cfg();
@@ -55,6 +70,10 @@ Linear::Call call_of(const char* who, const rmr_linear* layer, const rmr_linear_
     if (c->residual && !(c->residual == c->y && (c->rows == 1 || c->ldr == c->ldy)) &&
         y.meets(Range(c->residual, c->rows, cfg.out_features, c->rows > 1 ? c->ldr : 0, c->y_type)))
         fail(RMR_ERR_INVALID_ARGUMENT, "%s: y overlaps the residual and is not the residual itself", who);
+    const Range ws(c->workspace, c->workspace ? 1 : 0, (int64_t)(c->workspace_bytes / 2), 0, RMR_TYPE_F16);
+    if (ws.meets(y) || (!kept && ws.meets(Range(c->x, c->rows, cfg.in_features, c->rows > 1 ? c->ldx : 0, c->x_type))) ||
+        (c->residual && ws.meets(Range(c->residual, c->rows, cfg.out_features, c->rows > 1 ? c->ldr : 0, c->y_type))))
+        fail(RMR_ERR_INVALID_ARGUMENT, "%s: the workspace overlaps an operand", who);
     k.residual = c->residual, k.ldr = c->ldr, k.y = c->y, k.y_type = c->y_type, k.ldy = c->ldy;
     k.workspace = c->workspace, k.workspace_bytes = c->workspace_bytes;
     return k;
@@ -65,7 +84,7 @@ Linear::Call call_of(const char* who, const rmr_linear* layer, const rmr_linear_
 extern "C" {
 
 rmr_status rmr_feature_cache_create(int device, int64_t slots, int width, rmr_feature_cache** out) {
-    return guarded([&] {
+    return guarded_create([&] {
         if (!out || slots <= 0 || slots > (int64_t)1 << 40 || width <= 0 || width > RMR_FEATURE_MAX_WIDTH)
             fail(RMR_ERR_INVALID_ARGUMENT, "rmr_feature_cache_create: %lld slots of width %d", (long long)slots, width);
         *out = new rmr_feature_cache(device, slots, width);
@@ -91,6 +110,7 @@ rmr_status rmr_feature_cache_read(rmr_feature_cache* cache, const int64_t* slots
         if (!cache) fail(RMR_ERR_INVALID_ARGUMENT, "rmr_feature_cache_read: null cache");
         check_rows("rmr_feature_cache_read", "out", out, type, ld, n, cache->impl.width(), true);
         check_slots("rmr_feature_cache_read", slots, n);
+        check_apart("rmr_feature_cache_read", Range(out, n, cache->impl.width(), n > 1 ? ld : 0, type), slots, n);
         cache->impl.read(slots, n, out, type, n > 1 ? ld : 0, (hipStream_t)stream);
     });
 }
@@ -104,7 +124,7 @@ rmr_status rmr_detector_keep_feature(rmr_detector* det, const char* name, int im
 
 rmr_status rmr_linear_create(const rmr_linear_cfg* cfg, const void* weight, int weight_type, int64_t ldw, const float* bias, int mem,
                              void* stream, rmr_linear** out) {
-    return guarded([&] {
+    return guarded_create([&] {
         const char* who = "rmr_linear_create";
         if (!cfg || !out) fail(RMR_ERR_INVALID_ARGUMENT, "%s: null argument", who);
         if (cfg->in_features <= 0 || cfg->in_features > RMR_FEATURE_MAX_WIDTH || cfg->out_features <= 0 || cfg->out_features > 1 << 24)
@@ -144,6 +164,8 @@ rmr_status rmr_linear_run_kept(rmr_linear* layer, rmr_feature_cache* cache, cons
         if (!cache) fail(RMR_ERR_INVALID_ARGUMENT, "%s: null cache", who);
         Linear::Call c = call_of(who, layer, call, true);
         check_slots(who, slots, c.rows);
+        check_apart(who, Range(c.y, c.rows, layer->impl.out_features(), c.rows > 1 ? c.ldy : 0, c.y_type), slots, c.rows);
+        check_apart(who, Range(c.workspace, c.workspace ? 1 : 0, (int64_t)(c.workspace_bytes / 2), 0, RMR_TYPE_F16), slots, c.rows);
         const rmr_linear_cfg& cfg = layer->impl.cfg();
         if (cache->impl.width() != cfg.in_features)
             fail(RMR_ERR_INVALID_ARGUMENT, "%s: the cache's rows have %d values, the layer takes %d", who, cache->impl.width(), cfg.in_features);

@@ -36,7 +36,7 @@ struct WriteArgs {
     const int* owner;
     int64_t first, n_slots;
     int per_row;     // threads' chunks per row: pitch / values of a chunk
-    unsigned magic;  // ceil(2^32 / per_row): i / per_row for i < 2^16
+    unsigned magic;  // ceil(2^31 / per_row): i / per_row = i magic >> 31 while i per_row < 2^31
     int rows;        // rows of a group
     bool stream;     // pass the caches by
 };
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kThreads) void quantise_rows_kernel(WriteArgs a) {
         }
         const int chunks = rows * a.per_row;
         for (int i = tid; i < chunks; i += kThreads) {
-            const int r = (int)(((uint64_t)(unsigned)i * a.magic) >> 32);
+            const int r = (int)(((uint64_t)(unsigned)i * a.magic) >> 31);
             const int c = (i - r * a.per_row) * V;   // first value of the chunk
             int64_t to = a.first + r0 + r;
             if constexpr (DEST != DEST_RUN) to = later[r] ? -1 : dest[r];
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void read_rows_kernel(ReadArgs a) {
         const int rows = (int)(a.n - r0 < a.rows ? a.n - r0 : a.rows);
         const int chunks = rows * a.per_row;
         for (int i = threadIdx.x; i < chunks; i += kThreads) {
-            const int r = (int)(((uint64_t)(unsigned)i * a.magic) >> 32);
+            const int r = (int)(((uint64_t)(unsigned)i * a.magic) >> 31);
             const int c = (i - r * a.per_row) * V;
             const int64_t s = a.slots[r0 + r];
             float v[V];
@@ -174,7 +174,7 @@ int rows_per_group(int64_t n, int per_row, int cus) {
     return rows < 1 ? 1 : rows > kMaxRows ? kMaxRows : rows;
 }
 
-unsigned magic_of(int per_row) { return (unsigned)(((1ull << 32) + per_row - 1) / per_row); }
+unsigned magic_of(int per_row) { return (unsigned)(((1ull << 31) + per_row - 1) / per_row); }
 
 template <int DEST>
 void launch_write(DeviceCtx& ctx, hipStream_t s, int type, WriteArgs& a) {

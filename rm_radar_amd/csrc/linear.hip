@@ -113,27 +113,22 @@ __global__ __launch_bounds__(256) void pack_mx8_kernel(PackMx8Args a) {
 struct AlignArgs {
     const void* x;
     int64_t ld, n;
-    int width, per_row;
+    int width, per_row;   // 16-byte pieces of a row
+    unsigned magic;       // ceil(2^31 / per_row): i / per_row = i magic >> 31
+    int rows;             // rows of a workgroup
     unsigned char* out;
 };
 
 __global__ __launch_bounds__(256) void align_rows_kernel(AlignArgs a) {
-    const int64_t pieces = a.n * a.per_row;
-    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < pieces; p += (int64_t)gridDim.x * 256) {
-        const int64_t r = p / a.per_row;
-        const int c = (int)(p - r * a.per_row) * 8;
-        const unsigned short* src = (const unsigned short*)a.x + r * a.ld + c;
-        union {
-            u32x4 u;
-            unsigned short t[8];
-        } o;
-        if (c + 8 <= a.width) {
-            o.u = *(const u32x4_any*)src;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o.t[i] = c + i < a.width ? src[i] : (unsigned short)0;
+    const int64_t groups = (a.n + a.rows - 1) / a.rows;
+    for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
+        const int64_t r0 = g * a.rows;
+        const int pieces = (int)(a.n - r0 < a.rows ? a.n - r0 : a.rows) * a.per_row;
+        for (int i = threadIdx.x; i < pieces; i += 256) {
+            const int r = (int)(((uint64_t)(unsigned)i * a.magic) >> 31), c = (i - r * a.per_row) * 8;
+            const F16* src = (const F16*)a.x + (r0 + r) * a.ld + c;   // (any 16-bit type)
+            *(u32x4*)(a.out + (r0 * a.per_row + i) * 16) = load_words<F16>(src, a.width - c);
         }
-        *(u32x4*)(a.out + p * 16) = o.u;
     }
 }
 
@@ -1001,7 +996,7 @@ void launch_tile(LinearArgs a, int splits, hipStream_t s) {
     a.row_tiles = (a.rows + 16 * MT * WM - 1) / (16 * MT * WM);
     a.col_tiles = (a.groups + G * WN - 1) / (G * WN);
     const int64_t tiles = a.row_tiles * a.col_tiles;
-    if (tiles > 1 << 22) fail(RMR_ERR_INVALID_ARGUMENT, "linear: %lld tiles in one call", (long long)tiles);
+    if (tiles >= 1 << 24) fail(RMR_ERR_INVALID_ARGUMENT, "linear: %lld tiles in one call", (long long)tiles);
     linear_tile_kernel<FORMAT, MT, G, WM, WN, NB><<<dim3((unsigned)tiles, (unsigned)splits), 64 * WM * WN, 0, s>>>(a);
     RMR_HIP(hipGetLastError());
 }
@@ -1169,9 +1164,12 @@ void Linear::run(const Call& c) {
         launch_quantise_rows(ctx_, c.stream, c.x, cfg_.in_features, c.rows, r);
         a.x = r.data, a.x_pitch = r.pitch, a.x_scale = r.scale, a.x_scale_pitch = r.scale_pitch;
     } else if (p.x_bytes) {
-        const AlignArgs al{c.x.p, c.x.ld, c.rows, cfg_.in_features, ksteps_ * 8, (unsigned char*)c.workspace};
-        const int64_t blocks = (c.rows * al.per_row + 255) / 256;
-        align_rows_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, c.stream>>>(al);
+        const int per_row = ksteps_ * 8, rows = per_row < 1024 ? 1024 / per_row : 1;
+        const AlignArgs al{c.x.p, c.x.ld, c.rows, cfg_.in_features, per_row, (unsigned)(((1ull << 31) + per_row - 1) / per_row), rows, (unsigned char*)c.workspace};
+        const int64_t groups = (c.rows + rows - 1) / rows;
+        ProfScope align(ctx_.prof, c.stream, "align_rows", 0, 2.0 * c.rows * ksteps_ * kStepBytes);
+        align_rows_kernel<<<(unsigned)(groups < 65536 ? groups : 65536), 256, 0, c.stream>>>(al);
+        RMR_HIP(hipGetLastError());
         a.x = (const unsigned char*)c.workspace, a.x_pitch = (int64_t)ksteps_ * kStepBytes;
     } else {
         a.x = (const unsigned char*)c.x.p, a.x_pitch = c.ld_bytes();

@@ -2,7 +2,7 @@
 
 Operands are torch tensors on the GPU (float16, bfloat16 or float32, the last dimension packed, rows at any pitch and alignment);
 work is enqueued on torch's current stream of that device and nothing is waited for, so calls can be captured into a
-``torch.cuda.CUDAGraph``.  Outputs and workspaces come from torch's allocator.
+``torch.cuda.CUDAGraph``.  Outputs and workspaces come from torch's allocator.  Nothing is recorded for autograd.
 """
 from __future__ import annotations
 

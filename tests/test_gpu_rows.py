@@ -30,7 +30,7 @@ def make(rows, width, kind, seed, pad=0, offset=0, scale=1.0):
 # ---------------------------------------------------------------------------------------------------------------- cache
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("n,width,pad,offset", [(1, 1, 0, 0), (1, 576, 0, 0), (3, 31, 1, 1), (5, 33, 0, 3), (64, 128, 0, 0), (400, 576, 8, 0),
+@pytest.mark.parametrize("n,width,pad,offset", [(1, 1, 0, 0), (50, 1, 0, 0), (70, 3, 2, 1), (300, 4, 0, 0), (300, 8, 1, 0), (90, 9, 0, 0), (1, 576, 0, 0), (3, 31, 1, 1), (5, 33, 0, 3), (64, 128, 0, 0), (400, 576, 8, 0),
                                                 (17, 1001, 3, 5), (4097, 40, 0, 0), (6001, 257, 1, 0), (2, 65536, 0, 0)])
 def test_cache_write_and_read(rmr, kind, n, width, pad, offset):
     cap = n + 13
@@ -40,7 +40,8 @@ def test_cache_write_and_read(rmr, kind, n, width, pad, offset):
     cache.write(x, slots)
     want = ref.held(x)
     for out in ("f16", "bf16", "f32"):
-        assert torch.equal(cache.read(slots, dtype=KINDS[out]).cpu(), want.to(KINDS[out])), out
+        room = torch.full((n, width), float("nan"), dtype=KINDS[out], device="cuda")
+        assert torch.equal(cache.read(slots, out=room).cpu(), want.to(KINDS[out])), out
     rest = torch.ones(cap, dtype=torch.bool)
     rest[slots.cpu()] = False
     other = torch.arange(cap)[rest].cuda()
@@ -149,8 +150,9 @@ def test_read_leaves_what_is_between_rows(rmr):
 # --------------------------------------------------------------------------------------------------------------- linear
 
 SHAPES = [(1, 1, 1), (1, 64, 64), (1, 577, 130), (2, 27, 65), (5, 128, 16), (15, 1001, 77), (16, 256, 192), (17, 320, 64), (33, 72, 257),
-          (64, 512, 512), (65, 136, 129), (100, 640, 1000), (129, 264, 320), (200, 96, 33), (257, 1160, 260), (300, 65, 1100), (513, 200, 600),
-          (1500, 384, 1030), (2100, 1000, 250), (3001, 2200, 2900)]
+          (31, 300, 90), (32, 700, 4200), (33, 64, 64), (64, 512, 512), (65, 136, 129), (100, 640, 1000), (129, 264, 320), (200, 96, 33), (257, 1160, 260), (300, 65, 1100), (513, 200, 600),
+          (1500, 384, 1030), (2100, 1000, 250), (3001, 2200, 2900),
+          (100, 2100, 200), (40, 4300, 70), (64, 8200, 130)]
 
 
 @pytest.mark.parametrize("fmt", ["f16", "bf16", "mx8"])
@@ -168,6 +170,21 @@ def test_linear_exact_on_integers(rmr, fmt, m, k, n):
     got = layer(x.to(kind).cuda(), residual=r.cuda(), out_dtype=torch.float32)
     want = x.double() @ w.double().t() + b.double() + r.double()
     assert torch.equal(got.cpu().double(), want)
+
+
+@pytest.mark.parametrize("m,k,n", [(20, 5000, 4500), (500, 4200, 200), (700, 1000, 900), (3001, 2200, 2900)])
+def test_linear_exact_on_integers_with_16_bit_results(rmr, m, k, n):
+    """The block-scaled instructions: products of small whole numbers are not cut, so only the one rounding at the end is left."""
+    g = torch.Generator().manual_seed(m)
+    x = torch.randint(-3, 4, (m, k), generator=g).float()
+    w = torch.randint(-2, 3, (n, k), generator=g).float()
+    want = (x.double() @ w.double().t()).to(torch.bfloat16)
+    layer = rmr.Linear(w.cuda(), format="mx8")
+    assert torch.equal(layer(x.bfloat16().cuda()).cpu(), want)
+    cache = rmr.FeatureCache(m, k)
+    s = torch.randperm(m, generator=g).cuda()
+    cache.write(x.cuda(), s)
+    assert torch.equal(layer.kept(cache, s, out_dtype=torch.bfloat16).cpu(), want)
 
 
 @pytest.mark.parametrize("fmt,out", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("mx8", "bf16"), ("mx8", "f32"), ("mx8", "f16")])
@@ -308,12 +325,59 @@ def test_on_another_stream(rmr):
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_two_threads_on_one_layer(rmr):
+    """A layer is read-only: calls of different sizes from two threads on two streams do not disturb each other."""
+    import threading
+    layer = rmr.Linear(make(200, 1500, "f32", 85, scale=0.05), format="mx8", activation="silu")
+    xs = [make(m, 1500, "bf16", 86 + m) for m in (50, 400, 3000)]
+    want = [layer(x) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(order):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                for i in order:
+                    y = layer(xs[i])
+                    torch.cuda.current_stream().synchronize()
+                    if not torch.equal(y, want[i]):
+                        bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in ((0, 1, 2), (2, 0, 1))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_results_do_not_depend_on_the_run(rmr):
+    """No atomics in the sums: the same call gives the same bits, split over workgroups or not."""
+    for m, k, n in ((5, 4096, 4096), (64, 8192, 300), (300, 1000, 700)):
+        for fmt in ("bf16", "mx8"):
+            layer = rmr.Linear(make(n, k, "bf16", 87, scale=k ** -0.5), format=fmt)
+            x = make(m, k, "bf16", 88)
+            first = layer(x, out_dtype=torch.float32)
+            assert all(torch.equal(layer(x, out_dtype=torch.float32), first) for _ in range(5))
+
+
+def test_a_cache_that_does_not_fit_leaves_no_error_behind(rmr):
+    with pytest.raises(rmr.DeviceError):
+        rmr.FeatureCache(2 ** 39, 65536)
+    cache = rmr.FeatureCache(4, 40)
+    x = make(4, 40, "f16", 89)
+    s = torch.arange(4).cuda()
+    cache.write(x, s)
+    assert torch.equal(cache.read(s).cpu(), ref.held(x).half())
+
+
 def test_refusals(rmr):
     cache = rmr.FeatureCache(8, 64)
     f16 = rmr.Linear(make(32, 64, "f16", 91), format="f16")
     mx8 = rmr.Linear(make(32, 64, "f16", 91), format="mx8")
     x = make(4, 64, "f16", 92)
     s = torch.arange(4).cuda()
+    wide = torch.zeros(200, dtype=torch.int64, device="cuda")
     bad = rmr.InvalidArgument
     for call in (lambda: f16(x.bfloat16()), lambda: f16(x.float()), lambda: f16(x[:, :63]), lambda: f16(x.t()), lambda: f16(x.cpu()),
                  lambda: f16(x.double()), lambda: f16(x, residual=make(4, 32, "f32", 1)), lambda: f16(x, residual=make(3, 32, "f16", 1)),
@@ -323,7 +387,8 @@ def test_refusals(rmr):
                  lambda: f16.kept(cache, s), lambda: mx8.kept(rmr.FeatureCache(8, 65), s), lambda: mx8.kept(cache, s.int()), lambda: mx8.kept(cache, s.cpu()),
                  lambda: mx8.kept(cache, s[::2]), lambda: cache.write(x, s[:3]), lambda: cache.write(x[:, :32], s), lambda: cache.write(x.cpu(), s),
                  lambda: cache.write(x.long(), s), lambda: cache.read(s, out=torch.empty(3, 64, device="cuda")), lambda: cache.read(s.view(2, 2)),
-                 lambda: cache.read(s, out=torch.empty(1, 64, device="cuda").expand(4, 64)), lambda: cache.read(s, dtype=torch.int32)):
+                 lambda: cache.read(s, out=torch.empty(1, 64, device="cuda").expand(4, 64)), lambda: cache.read(wide[:4], out=wide.view(torch.float32)[:256].view(4, 64)),
+                 lambda: mx8.kept(cache, wide[:4], out=wide.view(torch.float16)[:128].view(4, 32)), lambda: cache.read(s, dtype=torch.int32)):
         with pytest.raises(bad):
             call()
     y = torch.empty(5, 32, dtype=torch.float16, device="cuda")
