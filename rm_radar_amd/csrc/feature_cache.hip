@@ -19,9 +19,10 @@ constexpr int64_t kMaxGrid = 65536;   // more row groups than this are walked
 // their slots in two passes over the list beforehand
 constexpr int64_t kScanRows = 4096;
 
-// the wide side of a call of more bytes than this passes the caches by (non-temporal), the cache's rows do not: 200000 scattered rows of
-// 1024 bf16 read in 130 us (137 without), written in 132 (152), of 1001 f32 read in 236 (292); smaller ones stay where the next
-// operator finds them
+// The wide side of a call of more bytes than this passes the caches by (non-temporal), the cache's rows do not.  Three states in turn:
+// 262144 scattered rows of 1024 bf16 read in 169 us (182 without), 200000 of 1001 f32 in 261 (301), written and read 363 (380) and 480
+// (531); writing alone gains where the rows fit the last-level cache (100000 x 576 f16 50, 59 without) and loses where they do not
+// (the first case 215, 201).  Smaller calls stay where the next operator finds them.
 constexpr int64_t kStreamBytes = 64 << 20;
 
 enum { DEST_RUN, DEST_SCAN, DEST_OWNER };
