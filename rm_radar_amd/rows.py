@@ -14,7 +14,6 @@ from ._lib import InvalidArgument, check, lib
 _FORMATS = {"f16": 0, "bf16": 1, "mx8": 2}
 _ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4}
 _types: dict = {}
-_devices: dict = {}
 
 
 def _torch():
@@ -65,13 +64,13 @@ def _slots(torch, t, device):
     return t.data_ptr(), t.shape[0]
 
 
-def _output(torch, shape, width, dtype, out, device):
-    """The caller's `out` or a new tensor [*shape, width]: (tensor, address, type, row pitch, rows)."""
+def _output(like, shape, width, dtype, out, device):
+    """The caller's `out` or a new tensor [*shape, width] beside `like`: (tensor, address, type, row pitch, rows)."""
     if out is None:
         kind = _types.get(dtype)
         if kind is None:
             _refuse(f"dtype {dtype} is not float16, bfloat16 or float32")
-        out = torch.empty((*shape, width), dtype=dtype, device=_devices.get(device) or _devices.setdefault(device, torch.device("cuda", device)))
+        out = like.new_empty((*shape, width), dtype=dtype)
         return out, out.data_ptr(), kind, width, None
     if dtype is not None and out.dtype != dtype:
         _refuse(f"out has dtype {out.dtype}, asked for {dtype}")
@@ -112,7 +111,7 @@ class FeatureCache:
         """The rows in ``slots`` as [n, width] of ``dtype`` (float16 by default) or into ``out``; zeros for slots that do not exist."""
         torch = _torch()
         sp, n = _slots(torch, slots, self.device)
-        out, p, kind, ld, m = _output(torch, (n,), self.width, dtype or (torch.float16 if out is None else None), out, self.device)
+        out, p, kind, ld, m = _output(slots, (n,), self.width, dtype or (torch.float16 if out is None else None), out, self.device)
         if m is not None and n != m:
             _refuse(f"{n} slots and {m} rows of out")
         check(self._lib.rmr_feature_cache_read(self._h, sp, n, p, kind, ld, _stream(torch, self.device)))
@@ -165,8 +164,8 @@ class Linear:
 
     __del__ = close
 
-    def _run(self, torch, x, x_kind, ldx, rows, lead, residual, out, out_dtype, cache, slots):
-        out, p, kind, ldy, n = _output(torch, lead, self.out_features, out_dtype, out, self.device)
+    def _run(self, torch, like, x, x_kind, ldx, rows, lead, residual, out, out_dtype, cache, slots):
+        out, p, kind, ldy, n = _output(like, lead, self.out_features, out_dtype, out, self.device)
         if n is not None and n != rows:
             _refuse(f"out has {n} rows, the call {rows}")
         r, ldr = None, 0
@@ -180,7 +179,7 @@ class Linear:
             need = C.c_size_t()
             check(self._lib.rmr_linear_workspace(self._h, at, cache is not None, C.byref(need)))
             if need.value:
-                space = torch.empty(need.value, dtype=torch.uint8, device=out.device)
+                space = out.new_empty(need.value, dtype=torch.uint8)
                 call.workspace, call.workspace_bytes = space.data_ptr(), need.value
         stream = _stream(torch, self.device)
         if cache is None:
@@ -194,11 +193,11 @@ class Linear:
         output, may be ``out`` itself."""
         torch = _torch()
         p, kind, ld, n = _rows(x, "x", self.in_features, self.device)
-        return self._run(torch, p, kind, ld, n, x.shape[:-1], residual, out, out_dtype or (x.dtype if out is None else None), None, None)
+        return self._run(torch, x, p, kind, ld, n, x.shape[:-1], residual, out, out_dtype or (x.dtype if out is None else None), None, None)
 
     def kept(self, cache, slots, residual=None, out=None, out_dtype=None):
         """The layer on the rows that ``cache`` holds in ``slots`` (int64 [n] on the GPU): [n, out_features] of ``out_dtype`` (float16 by
         default).  "mx8" layers only."""
         torch = _torch()
         sp, n = _slots(torch, slots, self.device)
-        return self._run(torch, None, 0, 0, n, (n,), residual, out, out_dtype or (torch.float16 if out is None else None), cache._h, sp)
+        return self._run(torch, slots, None, 0, 0, n, (n,), residual, out, out_dtype or (torch.float16 if out is None else None), cache._h, sp)
