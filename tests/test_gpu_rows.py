@@ -172,6 +172,16 @@ def test_linear_exact_on_integers(rmr, fmt, m, k, n):
     assert torch.equal(got.cpu().double(), want)
 
 
+@pytest.mark.parametrize("m,k", [(8193, 1001), (8300, 1001), (40001, 193), (8191, 1003), (300, 4101), (20000, 4101)])
+def test_linear_many_rows_of_odd_length(rmr, m, k):
+    """Rows that do not start at multiples of 16 bytes, few and many: whole numbers, exact."""
+    g = torch.Generator().manual_seed(m + k)
+    x = torch.randint(-3, 4, (m, k), generator=g).float().cuda()
+    w = torch.randint(-2, 3, (40, k), generator=g).float().cuda()
+    got = rmr.Linear(w, format="bf16")(x.bfloat16(), out_dtype=torch.float32)
+    assert torch.equal(got, x @ w.t())
+
+
 @pytest.mark.parametrize("m,k,n", [(20, 5000, 4500), (500, 4200, 200), (700, 1000, 900), (3001, 2200, 2900)])
 def test_linear_exact_on_integers_with_16_bit_results(rmr, m, k, n):
     """The block-scaled instructions: products of small whole numbers are not cut, so only the one rounding at the end is left."""
