@@ -41,9 +41,10 @@ void check_apart(const char* who, const Range& written, const int64_t* slots, in
     if (written.meets(Range(slots, 1, n * 4, 0, RMR_TYPE_F16))) fail(RMR_ERR_INVALID_ARGUMENT, "%s: the output overlaps slots", who);
 }
 
-// a handle that could not be made leaves no error behind for the next launch to report
+// a handle that could not be made leaves no error behind for the next launch to report, and the caller's device stays current
 template <class F>
 rmr_status guarded_create(F&& f) {
+    const DeviceKeeper keeper;
     const rmr_status s = guarded(std::forward<F>(f));
     if (s != RMR_OK) (void)hipGetLastError();
     return s;

@@ -218,7 +218,6 @@ void launch_quantise_rows(DeviceCtx& ctx, hipStream_t s, const RowSource& x, int
 }
 
 FeatureCache::FeatureCache(int device, int64_t slots, int width) : ctx_(device_ctx(device)), slots_(slots), width_(width) {
-    DeviceGuard guard(device);
     data_.alloc((size_t)(slots * mx8_pitch(width)));
     scale_.alloc((size_t)(slots * mx8_scale_pitch(width)));
     owner_.alloc((size_t)slots);

@@ -1070,7 +1070,6 @@ void launch_format(LinearArgs a, const Choice& c, hipStream_t s) {
 
 Linear::Linear(const rmr_linear_cfg& cfg, const void* weight, int weight_type, int64_t ldw, const float* bias, int mem, hipStream_t s)
     : ctx_(device_ctx(cfg.device)), cfg_(cfg) {
-    DeviceGuard guard(cfg.device);
     const int n = cfg.out_features, k = cfg.in_features;
     const bool mx8 = cfg.format == RMR_LINEAR_MX8;
     ksteps_ = mx8 ? (k + 127) / 128 : (k + 63) / 64;

@@ -32,6 +32,23 @@ class DeviceGuard {
     int before_ = 0, device_ = 0;
 };
 
+// gives the caller's device back whatever became current meanwhile: around the making of a handle, whose device_ctx() checks a device
+// and makes it current.  (Without a device there is none to give back.)
+class DeviceKeeper {
+   public:
+    DeviceKeeper() {
+        if (hipGetDevice(&before_) != hipSuccess) before_ = -1;
+    }
+    ~DeviceKeeper() {
+        if (before_ >= 0) (void)hipSetDevice(before_);
+    }
+    DeviceKeeper(const DeviceKeeper&) = delete;
+    DeviceKeeper& operator=(const DeviceKeeper&) = delete;
+
+   private:
+    int before_ = -1;
+};
+
 inline size_t type_bytes(int type) { return type == RMR_TYPE_F32 ? 4 : 2; }
 inline bool known_type(int type) { return type == RMR_TYPE_F16 || type == RMR_TYPE_BF16 || type == RMR_TYPE_F32; }
 inline int64_t mx8_pitch(int64_t width) { return (width + 127) / 128 * 128; }

@@ -1,0 +1,66 @@
+"""Host code of the feature cache and the linear layer on a stand-in HIP runtime of two devices (cpp/fake_hip.cpp): which device is
+current or waited for, what is refused and what is not.  No GPU takes part, kernels do nothing."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PRELUDE = """
+import ctypes as C, os, sys
+fake = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)          # before librmr.so: its calls go here
+fake.fake_hip_synced.restype = fake.fake_hip_launches.restype = C.c_long
+sys.path[:0] = [sys.argv[2], os.path.join(sys.argv[2], "tests")]
+import numpy as np
+import rm_radar_amd as rmr
+from rm_radar_amd import _lib
+L, OK, BAD = _lib.lib(), _lib.OK, _lib.ERR_INVALID_ARGUMENT
+assert rmr.device_count() == 2
+
+def current():
+    d = C.c_int()
+    fake.hipGetDevice(C.byref(d))
+    return d.value
+
+def cache(slots, width, device=0):
+    h = C.c_void_p()
+    return L.rmr_feature_cache_create(device, slots, width, C.byref(h)), h
+
+def layer(k, n, fmt=0, device=0):
+    h, w = C.c_void_p(), np.zeros((n, k), np.float32)
+    return L.rmr_linear_create(C.byref(_lib.LinearCfg(device, k, n, fmt, 0)), w.ctypes.data, 2, k, None, 0, None, C.byref(h)), h
+"""
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    import __graft_entry__ as g
+    from rm_radar_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        g.build()
+    so = str(tmp_path_factory.mktemp("fake") / "libfakehip.so")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                           os.path.join(ROOT, "tests", "cpp", "fake_hip.cpp"), "-o", so])
+    return so
+
+
+def run(fake, body, *args, **env):
+    res = subprocess.run([sys.executable, "-c", PRELUDE + body, fake, ROOT, *args], capture_output=True, text=True, timeout=300,
+                         env={**os.environ, **env})
+    assert res.returncode == 0, res.stdout + res.stderr
+
+
+def test_creation_leaves_the_callers_device(fake):
+    run(fake, """
+for mine, other in ((0, 1), (1, 0)):
+    fake.hipSetDevice(mine)
+    for device in (mine, other, other, 7):       # the first handle of a device, a further one, a device that is not there
+        for make in (lambda: cache(9, 40, device), lambda: layer(40, 9, 0, device), lambda: layer(40, 9, 2, device)):
+            status, h = make()
+            assert status == (OK if device < 2 else BAD) and current() == mine, (mine, device, status, current())
+    h = cache(9, 40, other)[1]
+    L.rmr_feature_cache_destroy(h)
+    assert current() == mine
+""")
