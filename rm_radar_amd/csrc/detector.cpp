@@ -330,7 +330,9 @@ void Detector::keep_feature(const std::string& name, int img, FeatureCache& cach
         fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: stage %s has %d channels, the cache's rows have %d values", name.c_str(), dims[2], cache.width());
     if (first_slot < 0 || first_slot > cache.slots() - n)
         fail(RMR_ERR_INVALID_ARGUMENT, "keep_feature: %lld rows from slot %lld do not fit %lld slots", (long long)n, (long long)first_slot, (long long)cache.slots());
-    // what other streams still read from the cache, or write to it, comes first: the caller has no hold on this one
+    // what other streams of the detector's device still read from the cache, or write to it, comes first: the caller has no hold on
+    // this one
+    DeviceGuard guard(ctx_.device);
     RMR_HIP(hipDeviceSynchronize());
     cache.write_run(RowSource{rows, RMR_TYPE_F16, ld}, first_slot, n, stream_);
     RMR_HIP(hipStreamSynchronize(stream_));

@@ -64,3 +64,20 @@ for mine, other in ((0, 1), (1, 0)):
     L.rmr_feature_cache_destroy(h)
     assert current() == mine
 """)
+
+
+def test_keep_feature_waits_for_the_detectors_device(fake, tmp_path):
+    run(fake, """
+import netutil
+from rm_radar_amd import weights as W
+pack = W.make_synthetic_pack(sys.argv[3], "s", 1, seed=3)
+det = rmr.Detector(pack, 1, (160, 160), 1, device=1, input_width=160, input_height=160)
+det.infer([netutil.test_image(0, 160, 160)])
+h, w, c = det.read_feature("model.21", 0).shape
+store = rmr.FeatureCache(h * w, c, device=1)
+fake.hipSetDevice(0)
+before = [fake.fake_hip_synced(d) for d in range(2)]
+det.keep_feature("model.21", store, 0)
+assert [fake.fake_hip_synced(d) for d in range(2)] == [before[0], before[1] + 1]
+assert current() == 0
+""", str(tmp_path / "car.rmrw"), RMR_ARENA_REUSE="0")
