@@ -144,8 +144,10 @@ void rmr_linear_destroy(rmr_linear* layer) { delete layer; }
 
 rmr_status rmr_linear_workspace(const rmr_linear* layer, const rmr_linear_call* call, int kept, size_t* bytes) {
     return guarded([&] {
-        if (!bytes) fail(RMR_ERR_INVALID_ARGUMENT, "rmr_linear_workspace: null argument");
-        Linear::Call c = call_of("rmr_linear_workspace", layer, call, kept != 0);
+        if (!bytes || !call) fail(RMR_ERR_INVALID_ARGUMENT, "rmr_linear_workspace: null argument");
+        rmr_linear_call asked = *call;   // whose workspace is still to be found
+        asked.workspace = nullptr, asked.workspace_bytes = 0;
+        Linear::Call c = call_of("rmr_linear_workspace", layer, &asked, kept != 0);
         c.kept = kept != 0;
         *bytes = layer->impl.workspace_bytes(c);
     });

@@ -81,3 +81,22 @@ det.keep_feature("model.21", store, 0)
 assert [fake.fake_hip_synced(d) for d in range(2)] == [before[0], before[1] + 1]
 assert current() == 0
 """, str(tmp_path / "car.rmrw"), RMR_ARENA_REUSE="0")
+
+
+def test_the_workspace_query_reads_no_workspace(fake):
+    run(fake, """
+h = layer(203, 96)[1]
+x, y, r = (np.zeros((400, 203), np.float16), np.zeros((400, 96), np.float16), np.zeros((400, 96), np.float16))
+need, again = C.c_size_t(), C.c_size_t()
+call = _lib.LinearCall(x.ctypes.data, 0, 203, 400, r.ctypes.data, 96, y.ctypes.data, 0, 96, None, 0)
+assert L.rmr_linear_workspace(h, C.byref(call), 0, C.byref(need)) == OK and need.value > 0
+for stale in (x, y, r):                         # what an earlier call may have left there
+    call.workspace, call.workspace_bytes = stale.ctypes.data, 1 << 40
+    assert L.rmr_linear_workspace(h, C.byref(call), 0, C.byref(again)) == OK and again.value == need.value
+    assert L.rmr_linear_run(h, C.byref(call), None) == BAD
+    call.workspace_bytes = need.value
+    assert L.rmr_linear_run(h, C.byref(call), None) == BAD
+space = np.zeros(need.value // 16 + 1, np.complex128)
+call.workspace = space.ctypes.data
+assert L.rmr_linear_run(h, C.byref(call), None) == OK
+""")
