@@ -21,14 +21,17 @@ struct Range {
     bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
 };
 
-// rows of `width` elements: type, element alignment, a row pitch whose products stay far inside 64 bits
+// no operand spans more than this: its end as an address, and every product on the way there, fits 63 bits
+constexpr int64_t kMaxSpan = (int64_t)1 << 56;
+
+// rows of `width` elements: type, element alignment, row pitch
 void check_rows(const char* who, const char* what, const void* p, int type, int64_t ld, int64_t rows, int64_t width, bool written) {
     if (!known_type(type)) fail(RMR_ERR_INVALID_ARGUMENT, "%s: unknown type %d of %s", who, type, what);
     if (rows < 0 || rows > kMaxRows) fail(RMR_ERR_INVALID_ARGUMENT, "%s: %lld rows", who, (long long)rows);
     if (rows == 0) return;
     if (!p) fail(RMR_ERR_INVALID_ARGUMENT, "%s: %s is null", who, what);
     if ((uintptr_t)p % type_bytes(type)) fail(RMR_ERR_INVALID_ARGUMENT, "%s: %s is not aligned to its elements", who, what);
-    if (rows > 1 && (ld < (written ? width : 0) || ld > (int64_t)1 << 31))
+    if (rows > 1 && (ld < (written ? width : 0) || ld > (int64_t)1 << 31 || (rows - 1) * ld > kMaxSpan / (int64_t)type_bytes(type)))
         fail(RMR_ERR_INVALID_ARGUMENT, "%s: rows of %s are %lld elements apart, %lld wide", who, what, (long long)ld, (long long)width);
 }
 

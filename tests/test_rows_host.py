@@ -100,3 +100,23 @@ space = np.zeros(need.value // 16 + 1, np.complex128)
 call.workspace = space.ctypes.data
 assert L.rmr_linear_run(h, C.byref(call), None) == OK
 """)
+
+
+def test_rows_that_span_more_than_an_address_are_refused(fake):
+    """(rows - 1) * pitch * element size past 2^63: the operands' ranges could not be compared."""
+    run(fake, """
+rows, far = (1 << 30) + 2, 1 << 31
+h, store = layer(8, 16)[1], cache(4, 8)[1]
+p, q = 1 << 44, 1 << 45                        # addresses that nobody follows
+for at in ((8, 16, far, 0), (8, 16, 16, far)):
+    ldx, ldy, wide = at[0], at[2], at[3]
+    call = _lib.LinearCall(p, 0, ldx, rows, q if wide else None, wide, q, 2, ldy, None, 0)
+    before = fake.fake_hip_launches()
+    assert L.rmr_linear_run(h, C.byref(call), None) == BAD and fake.fake_hip_launches() == before
+    assert b"elements apart" in L.rmr_last_error(), L.rmr_last_error()
+call = _lib.LinearCall(p, 0, far, (1 << 31) - 1, None, 0, q, 2, 16, None, 0)
+assert L.rmr_linear_run(h, C.byref(call), None) == BAD and b"elements apart" in L.rmr_last_error()
+assert L.rmr_feature_cache_write(store, p, 2, far, q, rows, None) == BAD and b"elements apart" in L.rmr_last_error()
+assert L.rmr_feature_cache_read(store, q, rows, p, 2, far, None) == BAD and b"elements apart" in L.rmr_last_error()
+assert L.rmr_feature_cache_read(store, q, 2, p, 2, far, None) == OK
+""")
