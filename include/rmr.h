@@ -460,7 +460,9 @@ rmr_status rmr_linear_create(const rmr_linear_cfg* cfg, const void* weight, int 
 void rmr_linear_destroy(rmr_linear* layer);
 /* One call's operands.  x: `rows` (below 2^31) rows of x_type, ldx elements apart (F16 / BF16: the layer's type; MX8: any).  y, and residual
  * if not NULL: rows of y_type, ldy / ldr elements apart.  residual may BE y (same address and ldr = ldy); apart from that y
- * overlaps no operand, and its rows do not overlap (ldy >= out_features).  Rows are x, or -- rmr_linear_run_kept, MX8
+ * overlaps no operand, and its rows do not overlap (ldy >= out_features).  Rows of one operand may lie between those of another
+ * as columns of one buffer do, at the same bytes from row to row; operands that reach into each other's span at different
+ * pitches are refused.  Rows are x, or -- rmr_linear_run_kept, MX8
  * layers -- the rows of a cache of width in_features in slots[0 .. rows) (DEVICE array; zeros where there is no such slot). */
 typedef struct {
     const void* x;

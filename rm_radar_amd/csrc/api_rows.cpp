@@ -10,15 +10,29 @@ namespace {
 
 constexpr int64_t kMaxRows = 0x7fffffff;
 
-// [p, p + bytes of `rows` rows) as addresses
+// the bytes of `rows` rows, `ld` elements apart; rows that touch or overlap are one long one
 struct Range {
-    uintptr_t lo = 0, hi = 0;
-    Range(const void* p, int64_t rows, int64_t width, int64_t ld, int type) {
-        if (!p || rows <= 0) return;
-        lo = (uintptr_t)p;
-        hi = lo + (uintptr_t)(((rows - 1) * ld + width) * (int64_t)type_bytes(type));
+    int64_t lo = 0, width = 0, pitch = 0, rows = 0;
+    Range(const void* p, int64_t n, int64_t w, int64_t ld, int type) {
+        if (!p || n <= 0) return;
+        const int64_t size = (int64_t)type_bytes(type);
+        lo = (int64_t)(uintptr_t)p, width = w * size, pitch = ld * size, rows = n;
+        if (rows > 1 && pitch <= width) width += (rows - 1) * pitch, rows = 1;
     }
-    bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+    int64_t hi() const { return lo + (rows - 1) * pitch + width; }
+    // whether a byte is in both.  Exact at one pitch, as columns of one wider buffer have; rows at two different pitches are taken to
+    // meet where their spans do.
+    bool meets(const Range& o) const {
+        if (!rows || !o.rows) return false;
+        if (rows == 1 && o.rows == 1) return lo < o.lo + o.width && o.lo < lo + width;
+        const int64_t step = rows > 1 ? pitch : o.pitch;
+        if (rows > 1 && o.rows > 1 && pitch != o.pitch) return lo < o.hi() && o.lo < hi();
+        // row j of o lies at d + k step from row i of this, k = j - i; the first k that does not end in front of it
+        const int64_t d = o.lo - lo, past = -o.width - d;
+        int64_t k = past / step - (past % step < 0) + 1;
+        if (k < 1 - rows) k = 1 - rows;
+        return k < o.rows && d + k * step < width;
+    }
 };
 
 // no operand spans more than this: its end as an address, and every product on the way there, fits 63 bits

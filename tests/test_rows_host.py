@@ -120,3 +120,57 @@ assert L.rmr_feature_cache_write(store, p, 2, far, q, rows, None) == BAD and b"e
 assert L.rmr_feature_cache_read(store, q, rows, p, 2, far, None) == BAD and b"elements apart" in L.rmr_last_error()
 assert L.rmr_feature_cache_read(store, q, 2, p, 2, far, None) == OK
 """)
+
+
+def test_overlap_goes_by_the_rows_not_by_what_lies_between(fake):
+    """y against x, the residual and the workspace, compared with the sets of bytes: columns of one buffer are apart.  Operands inside
+    each other's span at different pitches may be refused, but none that overlaps may pass."""
+    run(fake, """
+import random
+rng = random.Random(11)
+layers = {(k, n): layer(k, n)[1] for k in (8, 24) for n in (5, 16)}
+base = 1 << 44
+
+def taken(p, rows, width, ld):
+    return {p + 2 * (i * ld + j) for i in range(rows) for j in range(width)}
+
+seen = {True: 0, False: 0, "unsure": 0}
+for turn in range(6000):
+    (k, n), h = rng.choice(list(layers.items()))
+    rows = rng.choice((1, 2, 3, 7))
+    ldy = n + rng.choice((0, 1, 24, 40))
+    same = rng.random() < 0.7
+    other = rng.choice(("x", "residual", "workspace"))
+    y = base + 2 * rng.randrange(0, 120)
+    far = base + (1 << 20)
+    p = base + 2 * rng.randrange(0, 120)
+    x, ldx, r, ldr, ws, ws_bytes, single = far, k, None, 0, None, 0, rows == 1
+    if other == "x":
+        ldx = ldy if same else rng.choice((0, 3, k, k + 9))
+        x, them, single = p, taken(p, rows, k, ldx), single or ldx <= k
+    elif other == "residual":
+        ldr = ldy if same else rng.choice((0, 2, n, n + 7))
+        r, them, single = p, taken(p, rows, n, ldr), single or ldr <= n
+        if r == y and (rows == 1 or ldr == ldy):
+            them = set()                       # the residual may be y
+    else:
+        p -= p % 16
+        size = rng.choice((16, 64, 400))
+        ws, ws_bytes, them, single = p, size, taken(p, 1, size // 2, 0), True
+    meets = bool(them & taken(y, rows, n, ldy))
+    call = _lib.LinearCall(x, 0, ldx, rows, r, ldr, y, 0, ldy, ws, ws_bytes)
+    status = L.rmr_linear_run(h, C.byref(call), None)
+    sure = single or ldy == n or (ldx if other == "x" else ldr) == ldy
+    if meets or sure:
+        assert status == (BAD if meets else OK), (turn, other, rows, k, n, ldx, ldr, ldy, p - base, y - base, meets, L.rmr_last_error())
+        seen[meets] += 1
+    else:
+        assert status in (OK, BAD)
+        seen["unsure"] += 1
+assert min(seen.values()) > 20, seen
+# slots between the rows of an output that is written: 16 bytes of every 64, four slots are 32 bytes
+store = cache(9, 8)[1]
+for at in range(0, 256, 8):
+    want = BAD if {*range(at, at + 32)} & {i * 64 + j for i in range(4) for j in range(16)} else OK
+    assert L.rmr_feature_cache_read(store, base + at, 4, base, 0, 32, None) == want, at
+""")
