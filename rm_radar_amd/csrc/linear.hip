@@ -134,21 +134,38 @@ __global__ __launch_bounds__(256) void align_rows_kernel(AlignArgs a) {
 
 // ---------------------------------------------------------------------------------------------------------- the epilogue
 
-template <int ACT>
+// the activation of a result that is rounded to T behind it
+template <class T, int ACT>
 __device__ __forceinline__ float activate(float v) {
     constexpr float kLog2e = 1.44269504f;
     if constexpr (ACT == RMR_ACT_RELU) return v < 0.0f ? 0.0f : v;
     if constexpr (ACT == RMR_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
     if constexpr (ACT == RMR_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
     if constexpr (ACT == RMR_ACT_GELU) {
-        // v / 2 erfc(-v / sqrt 2) with Abramowitz & Stegun 7.1.26: erfc(z) = t (a1 + t (a2 + ...)) e^(-z z), t = 1 / (1 + p z), z >= 0,
-        // off by at most 1.5e-7 absolutely, which is 0.75e-7 |v| here; the coefficients are halved, z = |v| / sqrt 2
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(v), 1.0f));
-        float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-        q = fmaf(q, t, 0.5f * 1.421413741f);
-        q = fmaf(q, t, 0.5f * -0.284496736f);
-        q = fmaf(q, t, 0.5f * 0.254829592f);
-        q *= t * __builtin_amdgcn_exp2f(-0.5f * kLog2e * (v * v));   // erfc(|v| / sqrt 2) / 2
+        // v / 2 erfc(-v / sqrt 2) = v Phi(v), with Phi(-z) = e^(-z z / 2) g(z) for z = |v|, so that the negative side keeps its relative
+        // precision however small it gets.  g(z) = erfcx(z / sqrt 2) / 2 is t P(t), t = 1 / (1 + p z): the coefficients minimise the
+        // largest relative error for z <= 14.5, behind which the power is zero.  Degree 8 for an f32 result (2e-8; 4.5e-7 evaluated in
+        // f32); degree 5 is off by 5e-6, a hundredth of half a step of f16 (8192^3 bf16: 2 % less time than with degree 8).
+        constexpr bool kLong = sizeof(T) == 4;
+        const float t = __builtin_amdgcn_rcpf(fmaf(kLong ? 0.21f : 0.31f, fabsf(v), 1.0f));
+        float q;
+        if constexpr (kLong) {
+            q = fmaf(-0.0712944732f, t, 0.2818030221f);
+            q = fmaf(q, t, -0.3264901234f);
+            q = fmaf(q, t, 0.3449831350f);
+            q = fmaf(q, t, -0.0907701970f);
+            q = fmaf(q, t, 0.1234710871f);
+            q = fmaf(q, t, 0.0695700082f);
+            q = fmaf(q, t, 0.0850123999f);
+            q = fmaf(q, t, 0.0837151507f);
+        } else {
+            q = fmaf(-0.0739291299f, t, 0.1804503092f);
+            q = fmaf(q, t, 0.0157447480f);
+            q = fmaf(q, t, 0.1334297684f);
+            q = fmaf(q, t, 0.1204412802f);
+            q = fmaf(q, t, 0.1238607030f);
+        }
+        q *= t * __builtin_amdgcn_exp2f(-0.5f * kLog2e * (v * v));
         return v * (v < 0.0f ? q : 1.0f - q);
     }
     return v;
@@ -220,7 +237,7 @@ __device__ __forceinline__ void finish_full(const LinearArgs& a, Acc&& acc, cons
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const int k = p * V + i;
-                    o[i] = activate<ACT>(acc(std::integral_constant<int, m>{})[Q * 4 + (k >> 2)][k & 3] + bias[k >> 2][k & 3]);
+                    o[i] = activate<T, ACT>(acc(std::integral_constant<int, m>{})[Q * 4 + (k >> 2)][k & 3] + bias[k >> 2][k & 3]);
                     if (r) o[i] += to_f32(w.t[i]);
                 }
                 store_values<T>(y + p * V, V, o);
@@ -256,7 +273,7 @@ __device__ __forceinline__ void finish_edge(const LinearArgs& a, const float* sp
             for (int j = 0; j < 4; ++j) {
                 const f32x4 v = *(const f32x4*)(spill + 4 * j) + bias[j];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[(4 * j + i) / V][(4 * j + i) % V] = activate<decltype(act)::value>(v[i]);
+                for (int i = 0; i < 4; ++i) o[(4 * j + i) / V][(4 * j + i) % V] = activate<T, decltype(act)::value>(v[i]);
             }
         };
         switch (a.act) {
@@ -780,10 +797,10 @@ __device__ __forceinline__ void finish_quad(const LinearArgs& a, f32x4 v, int64_
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         switch (a.act) {
-            case RMR_ACT_RELU: v[i] = activate<RMR_ACT_RELU>(v[i]); break;
-            case RMR_ACT_SILU: v[i] = activate<RMR_ACT_SILU>(v[i]); break;
-            case RMR_ACT_GELU: v[i] = activate<RMR_ACT_GELU>(v[i]); break;
-            case RMR_ACT_SIGMOID: v[i] = activate<RMR_ACT_SIGMOID>(v[i]); break;
+            case RMR_ACT_RELU: v[i] = activate<T, RMR_ACT_RELU>(v[i]); break;
+            case RMR_ACT_SILU: v[i] = activate<T, RMR_ACT_SILU>(v[i]); break;
+            case RMR_ACT_GELU: v[i] = activate<T, RMR_ACT_GELU>(v[i]); break;
+            case RMR_ACT_SIGMOID: v[i] = activate<T, RMR_ACT_SIGMOID>(v[i]); break;
             default: break;
         }
     }
