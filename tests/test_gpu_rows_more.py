@@ -58,3 +58,76 @@ def test_gelu_is_right_in_relation_to_its_value(rmr, out, m, k, n):
     bound = bound + (y.abs() + bound) * ref.EPS[KINDS[out]] + ref.TINY[KINDS[out]]
     far = (got - y[:, None]).abs() - bound[:, None]
     assert far.max() <= 0, f"worst at v = {float(v[far.max(1).values.argmax()])}, by {float(far.max()):.3e}"
+
+
+# Held rows whose blocks have exponents of their own: x = i 2^(a(row) + c(block)), w = j 2^(b(feature) - c(block)) with small whole numbers i
+# and j.  Every product of one result is a whole number times 2^(a + b), so sums are exact, while a scale byte of another block, step, row or
+# feature changes the result by a power of two.
+
+def blocks_apart(m, k, n, seed, spread):
+    """f64 (x [m, k], w [n, k], x w^T), exact in every type of a cache's rows where |a| + |c| <= 9."""
+    g = torch.Generator().manual_seed(seed)
+    c = torch.randint(-spread, spread + 1, (-(-k // 32),), generator=g).double().repeat_interleave(32)[:k]
+    a = torch.randint(-3, 4, (m, 1), generator=g).double()
+    b = torch.randint(-3, 1, (n, 1), generator=g).double()
+    i, j = torch.randint(-3, 4, (m, k), generator=g).double(), torch.randint(-2, 3, (n, k), generator=g).double()
+    return i * torch.exp2(a + c), j * torch.exp2(b - c), (i @ j.t()) * torch.exp2(a + b.t())
+
+
+# few rows: 16 and 32, 16 and 32 features a workgroup; K split over workgroups; the three tiles, whole and at edges; K ending in a step
+@pytest.mark.parametrize("m,k,n", [(1, 577, 130), (16, 1000, 4200), (17, 320, 64), (32, 1300, 4200), (30, 640, 8200), (33, 72, 257), (300, 1160, 260), (64, 4300, 130),
+                                   (40, 8200, 70), (2100, 1400, 2600), (4100, 1200, 4200), (3001, 2200, 2900), (6000, 700, 1500), (512, 512, 512)])
+@pytest.mark.parametrize("src", ["f16", "bf16", "f32", "kept"])
+def test_scales_belong_to_their_blocks(rmr, m, k, n, src):
+    spread = 6 if src == "f16" else 20
+    x, w, want = blocks_apart(m, k, n, m + k + n, spread)
+    layer = rmr.Linear(w.float(), format="mx8")
+    if src == "kept":
+        cache = rmr.FeatureCache(m + 7, k)
+        s = torch.randperm(m + 7, generator=torch.Generator().manual_seed(m))[:m].cuda()
+        cache.write(x.float().cuda(), s)
+        call = lambda kind: layer.kept(cache, s, out_dtype=kind)                                       # noqa: E731
+    else:
+        call = lambda kind, x=x.to(KINDS[src]).cuda(): layer(x, out_dtype=kind)                       # noqa: E731
+    for kind in KINDS.values():
+        assert torch.equal(call(kind).cpu(), want.float().to(kind)), kind     # (f32 holds the sums exactly)
+
+
+def step_cut(x, w):
+    """How far the block-scaled instructions' sums of x [m, k] and w [n, k] may be off: within the 128 products that one of them takes,
+    each may be cut below 2^-13 of the largest."""
+    cut = torch.zeros(len(x), len(w), dtype=torch.float64)
+    for first in range(0, x.shape[1], 128):
+        a, b = x[:, first:first + 128].abs(), w[:, first:first + 128].abs()
+        top = torch.zeros_like(cut)
+        for p in range(a.shape[1]):
+            top = torch.maximum(top, a[:, p, None] * b[None, :, p])
+        cut += a.shape[1] * 2.0 ** -13 * top
+    return cut
+
+
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("m,k,n", [(16, 576, 64), (200, 576, 130), (64, 4300, 64), (300, 2048, 200)])
+def test_sums_of_held_rows_without_the_rounding_of_y(rmr, out, m, k, n):
+    """A residual that is the exact sum, rounded and negated, leaves the sum's own error in y, where half a step of y is small.
+
+    The sum is rounded (k + 2) times in f32 at most, the residual is exact, y is rounded once."""
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-6, 3, (m, -(-k // 32)), generator=g).float()).repeat_interleave(32, 1)[:, :k]
+    w = torch.randn(n, k, generator=g) * k ** -0.5
+    hx, hw = ref.held(x), ref.held(w)
+    s = hx @ hw.t()
+    r = -s.to(KINDS[out])
+    y = s + r.double()
+    u = 2.0 ** -24
+    bound = (k + 2) * 1.01 * u * (hx.abs() @ hw.abs().t()) + u * y.abs()
+    if out != "f32":
+        bound = bound + step_cut(hx, hw)
+    bound = bound + (y.abs() + bound) * ref.EPS[KINDS[out]] + ref.TINY[KINDS[out]]
+    layer = rmr.Linear(w, format="mx8")
+    got = layer(x.cuda(), residual=r.cuda(), out_dtype=KINDS[out]).cpu().double()
+    far = (got - y).abs() - bound
+    norm = ((hx * hx) @ (hw * hw).t()).sqrt()
+    print(f"{out} {m}x{k}x{n}: error / norm of the products: rms {float(((got - y) / norm).square().mean().sqrt()):.2e} max {float(((got - y).abs() / norm).max()):.2e}, "
+          f"bound / norm {float((bound / norm).median()):.2e}")
+    assert far.max() <= 0
