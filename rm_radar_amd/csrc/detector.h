@@ -34,7 +34,8 @@ class FrameStage {
 
 class Detector {
    public:
-    explicit Detector(const rmr_detector_cfg& cfg);
+    // shared (optional): the stream to work on, which outlives the detector
+    explicit Detector(const rmr_detector_cfg& cfg, hipStream_t shared = nullptr);
     ~Detector();
 
     // Detector::detect<T> (detector.h:117-134)
@@ -64,7 +65,7 @@ class Detector {
 
     rmr_detector_cfg cfg_;
     DeviceCtx& ctx_;
-    hipStream_t stream_ = nullptr;
+    hipStream_t stream_ = nullptr, own_stream_ = nullptr;
     hipEvent_t io_done_ = nullptr;   // behind the H2D copy of the last call's descriptor block (the pinned side is reused)
     std::unique_ptr<Yolov8> net_;
     FrameStage stage_;

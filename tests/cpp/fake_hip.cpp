@@ -11,16 +11,17 @@ namespace {
 
 constexpr int kDevices = 2;
 thread_local int current = 0;
-std::atomic<long> synced[kDevices], launches;
+std::atomic<long> synced[kDevices], launches, urgent;
 char names[64];   // what handles point at
 
 }  // namespace
 
 extern "C" {
 
-// for the tests: waits for the whole device, kernel launches so far
+// for the tests: waits for the whole device, kernel launches, streams of another priority than the default so far
 long fake_hip_synced(int device) { return synced[device]; }
 long fake_hip_launches() { return launches; }
+long fake_hip_priority_streams() { return urgent; }
 
 hipError_t hipGetDeviceCount(int* n) { return *n = kDevices, hipSuccess; }
 hipError_t hipGetDevice(int* d) { return *d = current, hipSuccess; }
@@ -35,7 +36,7 @@ hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600* p, int) {
     return hipSuccess;
 }
 hipError_t hipDeviceSynchronize() { return ++synced[current], hipSuccess; }
-hipError_t hipDeviceGetStreamPriorityRange(int* least, int* greatest) { return *least = *greatest = 0, hipSuccess; }
+hipError_t hipDeviceGetStreamPriorityRange(int* least, int* greatest) { return *least = 1, *greatest = -1, hipSuccess; }
 
 hipError_t hipMalloc(void** p, size_t n) { return (*p = std::calloc(1, n + 256)) ? hipSuccess : hipErrorOutOfMemory; }
 hipError_t hipFree(void* p) { return std::free(p), hipSuccess; }
@@ -51,7 +52,7 @@ hipError_t hipMemset(void* p, int v, size_t n) { return std::memset(p, v, n), hi
 hipError_t hipMemsetAsync(void* p, int v, size_t n, hipStream_t) { return std::memset(p, v, n), hipSuccess; }
 
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) { return *s = (hipStream_t)names, hipSuccess; }
-hipError_t hipStreamCreateWithPriority(hipStream_t* s, unsigned, int) { return *s = (hipStream_t)names, hipSuccess; }
+hipError_t hipStreamCreateWithPriority(hipStream_t* s, unsigned, int priority) { return urgent += priority != 0, *s = (hipStream_t)names, hipSuccess; }
 hipError_t hipStreamDestroy(hipStream_t) { return hipSuccess; }
 hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
 hipError_t hipStreamBeginCapture(hipStream_t, hipStreamCaptureMode) { return hipSuccess; }

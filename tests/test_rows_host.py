@@ -11,7 +11,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PRELUDE = """
 import ctypes as C, os, sys
 fake = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)          # before librmr.so: its calls go here
-fake.fake_hip_synced.restype = fake.fake_hip_launches.restype = C.c_long
+fake.fake_hip_synced.restype = fake.fake_hip_launches.restype = fake.fake_hip_priority_streams.restype = C.c_long
 sys.path[:0] = [sys.argv[2], os.path.join(sys.argv[2], "tests")]
 import numpy as np
 import rm_radar_amd as rmr
@@ -174,3 +174,17 @@ for at in range(0, 256, 8):
     want = BAD if {*range(at, at + 32)} & {i * 64 + j for i in range(4) for j in range(16)} else OK
     assert L.rmr_feature_cache_read(store, base + at, 4, base, 0, 32, None) == want, at
 """)
+
+
+def test_every_stream_has_the_default_priority(fake, tmp_path):
+    """Streams of different priorities at work beside each other have hung."""
+    run(fake, """
+import scenes
+from rm_radar_amd import weights as W
+cars = W.make_synthetic_pack(sys.argv[3] + "/car.rmrw", "s", 1, seed=3)
+armors = W.make_synthetic_pack(sys.argv[3] + "/armor.rmrw", "s", 12, seed=4)
+kept = [rmr.RobotDetector(cars, armors, (160, 160), 12, max_cars=2, opt_cars=2),
+        rmr.Locator(640, 640, scenes.K640, scenes.SAMPLE_L2C, np.eye(4, dtype=np.float32)), rmr.UploadRing(1, 4096), rmr.FeatureCache(4, 8)]
+assert layer(8, 16)[0] == OK
+assert fake.fake_hip_priority_streams() == 0
+""", str(tmp_path))
