@@ -439,10 +439,13 @@ rmr_status rmr_feature_cache_read(rmr_feature_cache* cache, const int64_t* slots
  * device's work in flight first; complete on return.  The call must have been of at most rmr_detector_chunk images. */
 rmr_status rmr_detector_keep_feature(rmr_detector* det, const char* name, int img, rmr_feature_cache* cache, int64_t first_slot);
 
-/* y[i] = act(W x[i] + bias) + residual[i] in one launch, accumulated in f32 and rounded once.
- * F16 / BF16: x and W of that type.  MX8: x and W held as a feature cache holds its rows, x quantised within the call; a 16-bit y
- * comes from the block-scaled matrix instructions, whose sums are good to about 2^-13 of the largest product, an f32 y from
- * products and sums in full f32, at half the rate. */
+/* y[i] = act(W x[i] + bias) + residual[i], accumulated in f32 and rounded once; the epilogue is part of the product's launch.
+ * (Rows above RMR_LINEAR_FEW_ROWS take a launch in front where MX8 quantises x or where 16-bit rows are not multiples of 16 bytes,
+ * and one behind where workgroups share a long K.)
+ * F16 / BF16: x and W of that type.  MX8: x and W held as a feature cache holds its rows, x quantised within the call.  A 16-bit y
+ * then comes from the block-scaled matrix instructions, which cut every product 13 bits below the largest of its group: sums are
+ * about 1.5e-5 of the norm of their products off, which a 16-bit y shows where they cancel to a few per cent of it.  An f32 y comes
+ * from products and sums in full f32, at half the rate (held values below 2^-126 with bf16's subnormal steps). */
 enum { RMR_LINEAR_F16 = 0, RMR_LINEAR_BF16 = 1, RMR_LINEAR_MX8 = 2 };
 enum { RMR_ACT_NONE = 0, RMR_ACT_RELU = 1, RMR_ACT_SILU = 2, RMR_ACT_GELU = 3 /* v / 2 erfc(-v / sqrt 2) */, RMR_ACT_SIGMOID = 4 };
 typedef struct {
@@ -458,7 +461,7 @@ typedef struct rmr_linear rmr_linear;
 rmr_status rmr_linear_create(const rmr_linear_cfg* cfg, const void* weight, int weight_type, int64_t ldw, const float* bias, int mem,
                              void* stream, rmr_linear** out);
 void rmr_linear_destroy(rmr_linear* layer);
-/* One call's operands.  x: `rows` (below 2^31) rows of x_type, ldx elements apart (F16 / BF16: the layer's type; MX8: any).  y, and residual
+/* One call's operands.  x: `rows` (below 2^31, and rows x features fewer than 2^24 tiles of 64 x 128) rows of x_type, ldx elements apart (F16 / BF16: the layer's type; MX8: any).  y, and residual
  * if not NULL: rows of y_type, ldy / ldr elements apart.  residual may BE y (same address and ldr = ldy); apart from that y
  * overlaps no operand, and its rows do not overlap (ldy >= out_features).  Rows of one operand may lie between those of another
  * as columns of one buffer do, at the same bytes from row to row; operands that reach into each other's span at different

@@ -21,8 +21,9 @@ constexpr int64_t kScanRows = 4096;
 
 // The wide side of a call of more bytes than this passes the caches by (non-temporal), the cache's rows do not.  Three states in turn:
 // 262144 scattered rows of 1024 bf16 read in 169 us (182 without), 200000 of 1001 f32 in 261 (301), written and read 363 (380) and 480
-// (531); writing alone gains where the rows fit the last-level cache (100000 x 576 f16 50, 59 without) and loses where they do not
-// (the first case 215, 201).  Smaller calls stay where the next operator finds them.
+// (531).  Most of that is the reads'.  A write alone gains where the rows fit the last-level cache (100000 x 576 f16 47 us, 56 without)
+// and loses where they do not (the first two cases 213 and 239, 200 and 225 without); with the read behind it that is made up for
+// (361 and 476, 361 and 482 without).  Smaller calls stay where the next operator finds them.
 constexpr int64_t kStreamBytes = 64 << 20;
 
 enum { DEST_RUN, DEST_SCAN, DEST_OWNER };

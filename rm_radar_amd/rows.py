@@ -123,7 +123,13 @@ class Linear:
 
     weight: [out_features, in_features], torch tensor (GPU or host) or numpy array; bias: [out_features] or None.  ``format``: "f16"
     / "bf16" (x and W of that type) or "mx8" (x and W in blocks of 8-bit values as a FeatureCache holds them; x of any type is
-    quantised within the call).  ``activation``: none, relu, silu, gelu (v / 2 erfc(-v / sqrt 2)), sigmoid."""
+    quantised within the call).  Weights of other types than float16, bfloat16 and float32 are rounded to float32 first.
+
+    An "mx8" layer's 16-bit results come from products cut 13 bits below the largest of their group: sums are about 1.5e-5 of
+    the norm of their products off, which shows where they cancel to a few per cent of it.  Float32 results (``out_dtype``) are summed
+    in full float32, at half the rate.
+
+    ``activation``: none, relu, silu, gelu (v / 2 erfc(-v / sqrt 2)), sigmoid."""
 
     def __init__(self, weight, bias=None, activation="none", format="f16", device=None):
         torch = _torch()
